@@ -510,6 +510,90 @@ QGEMV_API int qgemv_mg_synchronize(void* handle);
  * events (NULL: no-op). */
 QGEMV_API int qgemv_mg_destroy(void* handle);
 
+/* ---------------------------------------------------- mixture of experts
+ *
+ * For a few tokens n (a decode batch), with E experts of hidden size K and
+ * inner size F:
+ *   logits[n][e] = sum_k x[n][k] router[e][k]       (64-bit sums, one rounding to fp32)
+ *   ids[n][:], w[n][:]  = the top_k best experts and their weights
+ *   h[n][j] = w[n][j] * silu(gate_e x_n) * (up_e x_n),  e = ids[n][j]
+ *   y[n]    = sum_j down_e h[n][j]
+ * gate and up are [F, K], down is [K, F] per expert, in q8_0 or q4_0 (one
+ * format for gate and up, one for down); K % 32 == 0, F % 32 == 0, both at
+ * most 2^20.  Activations are rounded to 22-bit block fixed point as in the
+ * GEMVs.  x and y are fp32, bf16 or fp16 (QGEMV_F32 ...), y has x's type;
+ * row n of x is at x + n * ldx elements, row n of y at y + n * ldy.
+ *
+ * Limits: E (shared experts included) <= 1024, choices per token (shared
+ * experts included) <= 32, top_k <= router rows.  Any number of tokens; 64
+ * are taken at a time.
+ */
+#define QGEMV_F32 0
+#define QGEMV_BF16 1
+#define QGEMV_F16 2
+#define QGEMV_SOFTMAX 0
+#define QGEMV_SIGMOID 1
+
+/* Expert tiles: the layout that the kernels stream, made once per weight
+ * (16 rows x 128 columns in matrix-fragment order; columns padded to 128).
+ * Bytes of E experts' [rows, cols] matrices; gate and up together count as
+ * one matrix of 2 F rows.  0 when rows % 16 or cols % 32 is not 0. */
+QGEMV_API size_t qgemv_moe_tiles_bytes(int format, int64_t n_experts, int64_t rows, int64_t cols);
+/* Lays out E matrices [rows, cols] given as SoA planes (q, d), 16-byte and
+ * 2-byte aligned.  q2, d2 != NULL: a second set of the same shape, whose rows
+ * are interleaved with the first's (gate = q, up = q2; out holds 2 * rows). */
+QGEMV_API int qgemv_moe_tile(int format, const void* q, const void* d, const void* q2,
+                             const void* d2, int64_t n_experts, int64_t rows, int64_t cols,
+                             void* out, void* stream);
+
+typedef struct qgemv_expert_set {
+  int32_t format;       /* gate and up: QGEMV_Q8_0 or QGEMV_Q4_0 */
+  int32_t format_down;
+  int32_t n_experts;    /* all of them; the last n_shared take every token */
+  int32_t n_shared;
+  int64_t hidden;       /* K */
+  int64_t ffn;          /* F */
+  const void* gate_up;  /* tiles of gate and up, 16-byte aligned */
+  const void* down;     /* tiles of down, 16-byte aligned */
+} qgemv_expert_set;
+
+typedef struct qgemv_moe_router {
+  const void* w;        /* [n_experts][ldw], w_dtype */
+  int32_t w_dtype;
+  int32_t n_experts;    /* routed experts */
+  int64_t ldw;
+  const float* bias;    /* [n_experts] or NULL: added to the scores for the choice only */
+  int32_t top_k;
+  int32_t scoring;      /* QGEMV_SOFTMAX or QGEMV_SIGMOID of the logits */
+  int32_t normalize;    /* 1: the chosen weights are divided by their sum */
+  float scale;          /* then multiplied by this */
+} qgemv_moe_router;
+
+/* Routing alone: ids int32 [N][top_k] in descending order of score, weights
+ * fp32 [N][top_k].  Equal scores go to the lower index; a NaN score ranks
+ * below every number, and a token with a NaN logit gets NaN weights. */
+QGEMV_API int qgemv_moe_route(const qgemv_moe_router* router, const void* x, int dtype,
+                              int64_t ldx, int64_t n_tokens, int64_t hidden, int32_t* ids,
+                              float* weights, void* stream);
+/* Workspace bytes of a call with `slots` choices per token (top_k + n_shared
+ * for qgemv_moe_layer); 0 for sizes that the calls refuse. */
+QGEMV_API size_t qgemv_moe_workspace_bytes(int64_t n_tokens, int32_t slots, int64_t hidden,
+                                           int64_t ffn);
+/* The experts with the choice given: ids int32 [N][slots] (outside
+ * [0, n_experts): no expert, e.g. -1; the same expert twice: the sum of its
+ * weights), weights fp32 [N][slots].  A token without an expert gets zeros.
+ * n_shared is not used here.  workspace NULL: the stream's (allocated by the
+ * first such call, outside stream capture); else 16-byte aligned. */
+QGEMV_API int qgemv_moe_experts(const qgemv_expert_set* experts, const void* x, int dtype,
+                                int64_t ldx, const int32_t* ids, const float* weights,
+                                int32_t slots, int64_t n_tokens, void* y, int64_t ldy,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* The whole layer: routing over the first n_experts - n_shared experts, each
+ * shared expert with weight 1. */
+QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_router* router,
+                              const void* x, int dtype, int64_t ldx, int64_t n_tokens, void* y,
+                              int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,6 +45,23 @@ class StackRanksDesc(ctypes.Structure):
     _fields_ = [("nranks", ctypes.c_int32), ("rank", ctypes.c_int32), ("peer_y", ctypes.c_void_p)]
 
 
+class ExpertSet(ctypes.Structure):
+    """qgemv_expert_set of include/qgemv_b200.h."""
+    _fields_ = [("format", ctypes.c_int32), ("format_down", ctypes.c_int32),
+                ("n_experts", ctypes.c_int32), ("n_shared", ctypes.c_int32),
+                ("hidden", ctypes.c_int64), ("ffn", ctypes.c_int64),
+                ("gate_up", ctypes.c_void_p), ("down", ctypes.c_void_p)]
+
+
+class MoeRouter(ctypes.Structure):
+    """qgemv_moe_router of include/qgemv_b200.h."""
+    _fields_ = [("w", ctypes.c_void_p), ("w_dtype", ctypes.c_int32),
+                ("n_experts", ctypes.c_int32), ("ldw", ctypes.c_int64),
+                ("bias", ctypes.c_void_p), ("top_k", ctypes.c_int32),
+                ("scoring", ctypes.c_int32), ("normalize", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
 class QGemvError(RuntimeError):
     """A C-ABI call returned a non-zero qgemv_status."""
 
@@ -151,6 +168,15 @@ SIGNATURES = {
     "qgemv_quantize_aos": ([ctypes.c_int, _vp, _i64, _i64, _i64, _vp, _vp], ctypes.c_int),
     "qgemv_dequant_soa": ([ctypes.c_int, _vp, _vp, _vp, _i64, _i64, _vp], ctypes.c_int),
     "qgemv_repack": ([ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _i64, _i64, _vp], ctypes.c_int),
+    "qgemv_moe_tiles_bytes": ([ctypes.c_int, _i64, _i64, _i64], ctypes.c_size_t),
+    "qgemv_moe_tile": ([ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp],
+                       ctypes.c_int),
+    "qgemv_moe_route": ([_vp, _vp, ctypes.c_int, _i64, _i64, _i64, _vp, _vp, _vp], ctypes.c_int),
+    "qgemv_moe_workspace_bytes": ([_i64, _i32, _i64, _i64], ctypes.c_size_t),
+    "qgemv_moe_experts": ([_vp, _vp, ctypes.c_int, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _vp,
+                           ctypes.c_size_t, _vp], ctypes.c_int),
+    "qgemv_moe_layer": ([_vp, _vp, _vp, ctypes.c_int, _i64, _i64, _vp, _i64, _vp,
+                         ctypes.c_size_t, _vp], ctypes.c_int),
     "qgemv_roof_stream_read": ([_vp, _sz, _vp, _i32, _vp], ctypes.c_int),
     "qgemv_roof_bulk_read": ([_vp, _sz, _vp, _vp, _vp], ctypes.c_int),
     "qgemv_roof_d2d": ([_vp, _vp, _sz, _vp], ctypes.c_int),

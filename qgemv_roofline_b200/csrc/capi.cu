@@ -845,4 +845,162 @@ QGEMV_API int qgemv_roof_d2d(void* dst, const void* src, size_t bytes, void* str
   return OK;
 }
 
+QGEMV_API size_t qgemv_moe_tiles_bytes(int format, int64_t n_experts, int64_t rows, int64_t cols) {
+  if (check_fmt(format) || n_experts < 0 || n_experts > kMoeExperts || rows < 0 || rows % 16 ||
+      cols < 0 || cols % QK || rows > kMoeMaxDim * 2 || cols > kMoeMaxDim)
+    return 0;
+  return moe_tiles_bytes(format, n_experts, rows, cols);
+}
+
+QGEMV_API int qgemv_moe_tile(int format, const void* q, const void* d, const void* q2,
+                             const void* d2, int64_t n_experts, int64_t rows, int64_t cols,
+                             void* out, void* stream) {
+  if (int rc = check_fmt(format)) return rc;
+  if (n_experts < 0 || n_experts > kMoeExperts)
+    return set_error(ERR_ARG, "n_experts=%lld out of range [0, %d]", (long long)n_experts, kMoeExperts);
+  if (rows < 0 || cols < 0 || rows % QK || cols % QK)
+    return set_error(ERR_SHAPE, "rows=%lld and cols=%lld must be multiples of 32", (long long)rows,
+                     (long long)cols);
+  if (rows > kMoeMaxDim || cols > kMoeMaxDim)
+    return set_error(ERR_UNSUPPORTED, "expert matrices of up to 2^20 rows and columns");
+  if (!n_experts || !rows || !cols) return OK;
+  if (!q || !d || !out || (q2 && !d2)) return set_error(ERR_NULL, "q, d and out must not be NULL");
+  if (misaligned(q, 16) || misaligned(q2, 16) || misaligned(out, 16) || misaligned(d, 2) ||
+      misaligned(d2, 2))
+    return set_error(ERR_ALIGN, "quants and out must be 16-byte, scales 2-byte aligned");
+  return moe_tile(format, q, d, q2, d2, n_experts, rows, cols, out, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+int check_moe_x(const void* x, int dtype, int64_t ldx, int64_t N, int64_t K) {
+  if (dtype < 0 || dtype > 2) return set_error(ERR_ARG, "dtype must be 0, 1 or 2, got %d", dtype);
+  if (N < 0 || K < 1) return set_error(ERR_SHAPE, "n_tokens=%lld hidden=%lld", (long long)N, (long long)K);
+  if (N >= kMaxDim || K > kMoeMaxDim)
+    return set_error(ERR_UNSUPPORTED, "n_tokens must be below 2^31 and hidden at most 2^20");
+  if (N == 0) return OK;
+  if (!x) return set_error(ERR_NULL, "x must not be NULL");
+  if (misaligned(x, dtype == 0 ? 4 : 2)) return set_error(ERR_ALIGN, "x must be aligned to its elements");
+  if (ldx < (N > 1 ? K : 0)) return set_error(ERR_SHAPE, "ldx=%lld < hidden=%lld", (long long)ldx, (long long)K);
+  return OK;
+}
+
+int check_router(const qgemv_moe_router* r, int64_t K, MoeRoute& out) {
+  if (!r) return set_error(ERR_NULL, "router must not be NULL");
+  if (r->w_dtype < 0 || r->w_dtype > 2)
+    return set_error(ERR_ARG, "w_dtype must be 0, 1 or 2, got %d", r->w_dtype);
+  if (r->n_experts < 1 || r->n_experts > kMoeExperts)
+    return set_error(ERR_ARG, "n_experts=%d out of range [1, %d]", r->n_experts, kMoeExperts);
+  if (r->top_k < 1 || r->top_k > r->n_experts || r->top_k > kMoeSlots)
+    return set_error(ERR_ARG, "top_k=%d out of range [1, min(%d experts, %d)]", r->top_k, r->n_experts,
+                     kMoeSlots);
+  if (r->scoring != 0 && r->scoring != 1)
+    return set_error(ERR_ARG, "scoring must be 0 (softmax) or 1 (sigmoid), got %d", r->scoring);
+  if (!r->w) return set_error(ERR_NULL, "the router's weights must not be NULL");
+  if (misaligned(r->w, r->w_dtype == 0 ? 4 : 2) || misaligned(r->bias, 4))
+    return set_error(ERR_ALIGN, "the router's weights must be aligned to their elements, its bias to 4 bytes");
+  if (r->ldw < (r->n_experts > 1 ? K : 0))
+    return set_error(ERR_SHAPE, "ldw=%lld < hidden=%lld", (long long)r->ldw, (long long)K);
+  out.w = r->w;
+  out.wdt = r->w_dtype;
+  out.ldw = r->ldw;
+  out.bias = r->bias;
+  out.E = r->n_experts;
+  out.k = r->top_k;
+  out.scoring = r->scoring;
+  out.normalize = r->normalize != 0;
+  out.scale = r->scale;
+  return OK;
+}
+
+int moe_entry(const qgemv_expert_set* m, const qgemv_moe_router* router, const void* x, int dtype,
+              int64_t ldx, const int32_t* ids, const float* weights, int32_t slots, int64_t N,
+              void* y, int64_t ldy, void* ws, size_t ws_bytes, void* stream) {
+  if (!m) return set_error(ERR_NULL, "experts must not be NULL");
+  if (int rc = check_fmt(m->format)) return rc;
+  if (int rc = check_fmt(m->format_down)) return rc;
+  if (m->n_experts < 1 || m->n_experts > kMoeExperts || m->n_shared < 0 || m->n_shared > m->n_experts)
+    return set_error(ERR_ARG, "n_experts=%d (of them n_shared=%d) out of range [1, %d]", m->n_experts,
+                     m->n_shared, kMoeExperts);
+  if (m->hidden < QK || m->ffn < QK || m->hidden % QK || m->ffn % QK)
+    return set_error(ERR_SHAPE, "hidden=%lld and ffn=%lld must be multiples of 32", (long long)m->hidden,
+                     (long long)m->ffn);
+  if (m->hidden > kMoeMaxDim || m->ffn > kMoeMaxDim)
+    return set_error(ERR_UNSUPPORTED, "hidden and ffn must be at most 2^20");
+  if (int rc = check_moe_x(x, dtype, ldx, N, m->hidden)) return rc;
+  MoeRoute route;
+  if (router) {
+    if (int rc = check_router(router, m->hidden, route)) return rc;
+    if (router->n_experts != m->n_experts - m->n_shared)
+      return set_error(ERR_SHAPE, "the router has %d rows for %d routed experts", router->n_experts,
+                       m->n_experts - m->n_shared);
+    slots = router->top_k + m->n_shared;
+  }
+  if (slots < 1 || slots > kMoeSlots)
+    return set_error(ERR_ARG, "%d choices per token, out of range [1, %d]", slots, kMoeSlots);
+  if (N == 0) return OK;
+  if (!y || !m->gate_up || !m->down) return set_error(ERR_NULL, "y and the tiles must not be NULL");
+  if (!router && (!ids || !weights)) return set_error(ERR_NULL, "ids and weights must not be NULL");
+  if (misaligned(m->gate_up, 16) || misaligned(m->down, 16) || misaligned(y, dtype == 0 ? 4 : 2) ||
+      misaligned(ids, 4) || misaligned(weights, 4))
+    return set_error(ERR_ALIGN, "tiles must be 16-byte aligned, ids and weights 4-byte, y to its elements");
+  if (ldy < (N > 1 ? m->hidden : 0))
+    return set_error(ERR_SHAPE, "ldy=%lld < hidden=%lld", (long long)ldy, (long long)m->hidden);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t need = moe_workspace_bytes(N, slots, m->hidden, m->ffn);
+  if (ws) {
+    if (ws_bytes < need)
+      return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, ws_bytes);
+    if (misaligned(ws, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
+  } else if (int rc = stream_workspace(st, need, &ws)) {
+    return rc;
+  }
+  MoeExperts e;
+  e.fmt = m->format;
+  e.fmt_down = m->format_down;
+  e.E = m->n_experts;
+  e.K = m->hidden;
+  e.F = m->ffn;
+  e.gate_up = m->gate_up;
+  e.down = m->down;
+  return moe_experts(e, router ? &route : nullptr, x, dtype, ldx, ids, weights, slots, N, y, ldy, ws, st);
+}
+}  // namespace
+
+QGEMV_API int qgemv_moe_route(const qgemv_moe_router* router, const void* x, int dtype,
+                              int64_t ldx, int64_t n_tokens, int64_t hidden, int32_t* ids,
+                              float* weights, void* stream) {
+  if (int rc = check_moe_x(x, dtype, ldx, n_tokens, hidden)) return rc;
+  MoeRoute r;
+  if (int rc = check_router(router, hidden, r)) return rc;
+  if (n_tokens == 0) return OK;
+  if (!ids || !weights) return set_error(ERR_NULL, "ids and weights must not be NULL");
+  if (misaligned(ids, 4) || misaligned(weights, 4))
+    return set_error(ERR_ALIGN, "ids and weights must be 4-byte aligned");
+  return moe_route(r, x, dtype, ldx, n_tokens, hidden, ids, weights, static_cast<cudaStream_t>(stream));
+}
+
+QGEMV_API size_t qgemv_moe_workspace_bytes(int64_t n_tokens, int32_t slots, int64_t hidden,
+                                           int64_t ffn) {
+  if (n_tokens < 1 || slots < 1 || slots > kMoeSlots || hidden < QK || ffn < QK || hidden % QK ||
+      ffn % QK || hidden > kMoeMaxDim || ffn > kMoeMaxDim)
+    return 0;
+  return moe_workspace_bytes(n_tokens, slots, hidden, ffn);
+}
+
+QGEMV_API int qgemv_moe_experts(const qgemv_expert_set* experts, const void* x, int dtype,
+                                int64_t ldx, const int32_t* ids, const float* weights,
+                                int32_t slots, int64_t n_tokens, void* y, int64_t ldy,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return moe_entry(experts, nullptr, x, dtype, ldx, ids, weights, slots, n_tokens, y, ldy,
+                   workspace, workspace_bytes, stream);
+}
+
+QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_router* router,
+                              const void* x, int dtype, int64_t ldx, int64_t n_tokens, void* y,
+                              int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!router) return set_error(ERR_NULL, "router must not be NULL");
+  return moe_entry(experts, router, x, dtype, ldx, nullptr, nullptr, 0, n_tokens, y, ldy,
+                   workspace, workspace_bytes, stream);
+}
+
 }  // extern "C"

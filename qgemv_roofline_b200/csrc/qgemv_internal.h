@@ -167,4 +167,36 @@ int roof_stream_read(const void* buf, size_t bytes, uint32_t* sink, int blocks_p
 int roof_bulk_read(const void* buf, size_t bytes, uint32_t* sink, int* status,
                    cudaStream_t st);
 
+// Mixture of experts (moe.cu).  A pass takes up to kMoeTokens tokens; longer
+// calls are split.  dtypes: 0 fp32, 1 bf16, 2 fp16.
+constexpr int kMoeTokens = 64;
+constexpr int kMoeSlots = 32;     // choices per token, the shared experts among them
+constexpr int kMoeExperts = 1024;
+constexpr int64_t kMoeMaxDim = (int64_t)1 << 20;  // hidden and inner size
+struct MoeRoute {
+  const void* w = nullptr;  // router [E][ldw]
+  int wdt = 0;
+  int64_t ldw = 0;
+  const float* bias = nullptr;  // [E], added to the scores for the choice only
+  int E = 0, k = 0, scoring = 0, normalize = 1;  // scoring: 0 softmax, 1 sigmoid
+  float scale = 1.0f;
+};
+struct MoeExperts {
+  int fmt = 0, fmt_down = 0;  // 8 or 4: gate and up; down
+  int E = 0;                  // experts, the shared ones among them
+  int64_t K = 0, F = 0;
+  const void* gate_up = nullptr;
+  const void* down = nullptr;
+};
+size_t moe_tiles_bytes(int fmt, int64_t E, int64_t rows, int64_t cols);
+int moe_tile(int fmt, const void* q, const void* d, const void* q2, const void* d2, int64_t E,
+             int64_t rows, int64_t cols, void* out, cudaStream_t st);
+size_t moe_workspace_bytes(int64_t N, int slots, int64_t K, int64_t F);
+int moe_route(const MoeRoute& c, const void* x, int xdt, int64_t ldx, int64_t N, int64_t K,
+              int* ids, float* weights, cudaStream_t st);
+// route == nullptr: ids and weights are the caller's; else they are computed.
+int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int xdt, int64_t ldx,
+                const int* ids, const float* weights, int slots, int64_t N, void* y, int64_t ldy,
+                void* ws, cudaStream_t st);
+
 }  // namespace qg

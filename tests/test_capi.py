@@ -155,3 +155,60 @@ def test_multi_gpu_handle_validation():
     assert lib.qgemv_mg_gemv(None, None, None, 1, 1, None) == 1
     assert lib.qgemv_mg_synchronize(None) == 1
     assert lib.qgemv_mg_destroy(None) == 0
+
+
+def test_moe_validation():
+    L = _lib
+    r = L.MoeRouter(FAKE, 0, 8, 64, None, 2, 0, 1, 1.0)
+    e = L.ExpertSet(8, 4, 9, 1, 64, 32, FAKE, FAKE)
+    R, S = ctypes.byref(r), ctypes.byref(e)
+
+    def layer(x=FAKE, dt=0, ldx=64, n=2, y=FAKE, ldy=64, ws=FAKE, nb=1 << 30):
+        return rc("qgemv_moe_layer", S, R, x, dt, ldx, n, y, ldy, ws, nb, None)
+
+    assert rc("qgemv_moe_layer", None, R, FAKE, 0, 64, 2, FAKE, 64, FAKE, 1 << 30, None) == 1
+    assert rc("qgemv_moe_layer", S, None, FAKE, 0, 64, 2, FAKE, 64, FAKE, 1 << 30, None) == 1
+    assert layer(n=0) == 0
+    assert layer(x=None) == 1 and layer(y=None) == 1
+    assert layer(dt=3) == 7 and layer(n=-1) == 2
+    assert layer(ldx=63) == 2 and layer(ldy=63) == 2
+    assert layer(x=FAKE + 2) == 3 and layer(y=FAKE + 2) == 3 and layer(ws=FAKE + 8) == 3
+    assert layer(nb=16) == 7 and "workspace" in L.last_error()
+
+    def with_(s, **kw):
+        old = {k: getattr(s, k) for k in kw}
+        for k, v in kw.items():
+            setattr(s, k, v)
+        got = layer()
+        for k, v in old.items():
+            setattr(s, k, v)
+        return got
+
+    assert with_(r, top_k=0) == 7 and with_(r, top_k=9) == 7 and with_(r, scoring=2) == 7
+    assert with_(r, w=None) == 1 and with_(r, w=FAKE + 2) == 3 and with_(r, bias=FAKE + 1) == 3
+    assert with_(r, n_experts=7) == 2          # not the routed experts
+    assert with_(r, n_experts=1025) == 7 and with_(r, ldw=63) == 2 and with_(r, w_dtype=5) == 7
+    assert with_(e, format=5) == 7 and with_(e, format_down=3) == 7
+    assert with_(e, n_experts=0) == 7 and with_(e, n_shared=-1) == 7 and with_(e, n_experts=1025) == 7
+    assert with_(e, hidden=48) == 2 and with_(e, ffn=0) == 2 and with_(e, ffn=(1 << 20) + 32) == 5
+    assert with_(e, gate_up=None) == 1 and with_(e, down=FAKE + 4) == 3
+
+    def experts(ids=FAKE, w=FAKE, slots=2):
+        return rc("qgemv_moe_experts", S, FAKE, 0, 64, ids, w, slots, 2, FAKE, 64, FAKE, 1 << 30, None)
+
+    assert experts(ids=None) == 1 and experts(w=None) == 1 and experts(ids=FAKE + 2) == 3
+    assert experts(slots=0) == 7 and experts(slots=33) == 7
+    assert rc("qgemv_moe_route", R, FAKE, 0, 64, 2, 64, None, FAKE, None) == 1
+    assert rc("qgemv_moe_route", R, FAKE, 0, 64, 2, 64, FAKE, FAKE + 2, None) == 3
+    assert rc("qgemv_moe_route", R, FAKE, 0, 64, 2, 0, FAKE, FAKE, None) == 2
+    assert rc("qgemv_moe_route", R, FAKE, 0, 64, 0, 64, None, None, None) == 0
+    assert rc("qgemv_moe_tile", 8, FAKE, FAKE, None, None, 2, 48, 64, FAKE, None) == 2
+    assert rc("qgemv_moe_tile", 8, FAKE, FAKE, FAKE, None, 2, 64, 64, FAKE, None) == 1
+    assert rc("qgemv_moe_tile", 8, FAKE + 8, FAKE, None, None, 2, 64, 64, FAKE, None) == 3
+    assert rc("qgemv_moe_tile", 4, FAKE, FAKE, None, None, 1025, 64, 64, FAKE, None) == 7
+    assert rc("qgemv_moe_tile", 4, None, None, None, None, 0, 64, 64, None, None) == 0
+    # 16 rows x 128 columns: quants and 64 scales
+    assert _lib.lib().qgemv_moe_tiles_bytes(8, 3, 32, 160) == 3 * 2 * 2 * (2048 + 128)
+    assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 32, 160) == 3 * 2 * 2 * (1024 + 128)
+    assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 40, 160) == 0
+    assert _lib.lib().qgemv_moe_workspace_bytes(1, 33, 64, 64) == 0
