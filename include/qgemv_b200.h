@@ -594,6 +594,37 @@ QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_r
                               const void* x, int dtype, int64_t ldx, int64_t n_tokens, void* y,
                               int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------- int8 products
+ *
+ * y[n][m] = (sum_k xq[n][k] wq[m][k]) * xs[n] * ws[m] (+ bias[m])
+ * with int8 rows and one fp32 scale per token n and per channel m, any number
+ * of tokens.  The sum is exact (int32); it is rounded to fp32, multiplied by
+ * xs, then by ws, the bias is added, and the result is rounded to y's type
+ * (QGEMV_F32, QGEMV_BF16 or QGEMV_F16).  K % 16 == 0, 16 <= K < 2^17; xq and
+ * wq 16-byte aligned with row strides (in bytes) that are multiples of 16.
+ * Row n of y is at y + n * ldy elements.
+ */
+
+/* One scale per row: scales = max |x| / 127, q = rint(x / scales) (fp32
+ * division and rounding), for activations and weights alike.  An all-zero row
+ * gets scale 0 and zeros, a row with a NaN or an infinity scale NaN and zeros
+ * (its products are NaN).  Any K; row n of x at x + n * ldx elements, of q at
+ * q + n * ldq bytes. */
+QGEMV_API int qgemv_int8_quantize(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K,
+                                  void* q, int64_t ldq, float* scales, void* stream);
+QGEMV_API int qgemv_int8_matmul(const void* xq, const float* xs, int64_t ldx, const void* wq,
+                                const float* ws, int64_t ldw, const float* bias, int64_t N,
+                                int64_t M, int64_t K, void* y, int y_dtype, int64_t ldy,
+                                void* stream);
+/* The two together: x (fp32, bf16 or fp16) is rounded per token into the
+ * workspace (16-byte aligned; NULL: the stream's, allocated by the first such
+ * call outside stream capture), then multiplied. */
+QGEMV_API size_t qgemv_int8_linear_workspace_bytes(int64_t N, int64_t K);
+QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const void* wq,
+                                const float* ws, int64_t ldw, const float* bias, int64_t N,
+                                int64_t M, int64_t K, void* y, int y_dtype, int64_t ldy,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

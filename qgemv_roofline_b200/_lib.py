@@ -177,6 +177,12 @@ SIGNATURES = {
                            ctypes.c_size_t, _vp], ctypes.c_int),
     "qgemv_moe_layer": ([_vp, _vp, _vp, ctypes.c_int, _i64, _i64, _vp, _i64, _vp,
                          ctypes.c_size_t, _vp], ctypes.c_int),
+    "qgemv_int8_quantize": ([_vp, ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _vp], ctypes.c_int),
+    "qgemv_int8_matmul": ([_vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, ctypes.c_int,
+                           _i64, _vp], ctypes.c_int),
+    "qgemv_int8_linear_workspace_bytes": ([_i64, _i64], ctypes.c_size_t),
+    "qgemv_int8_linear": ([_vp, ctypes.c_int, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp,
+                           ctypes.c_int, _i64, _vp, ctypes.c_size_t, _vp], ctypes.c_int),
     "qgemv_roof_stream_read": ([_vp, _sz, _vp, _i32, _vp], ctypes.c_int),
     "qgemv_roof_bulk_read": ([_vp, _sz, _vp, _vp, _vp], ctypes.c_int),
     "qgemv_roof_d2d": ([_vp, _vp, _sz, _vp], ctypes.c_int),

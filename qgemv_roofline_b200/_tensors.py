@@ -1,0 +1,83 @@
+"""What the multi-type operators (moe, int8) share on the host: argument checks
+and the stream and workspace of a call.  These run on every call of a decode
+step, beside kernels of a few microseconds, so they keep to a few attribute
+reads and no temporary objects."""
+
+from __future__ import annotations
+
+import functools
+
+import torch
+
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def on_device_of_x(fn):
+    """Runs ``fn(x, ...)`` with the device of ``x`` current."""
+    @functools.wraps(fn)
+    def wrapper(x, *args, **kwargs):
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise ValueError("x must be a CUDA tensor")
+        if x.get_device() == torch.cuda.current_device():
+            return fn(x, *args, **kwargs)
+        with torch.cuda.device(x.device):
+            return fn(x, *args, **kwargs)
+    return wrapper
+
+
+def rows_of(x: torch.Tensor, K: int):
+    """x ([K] or [N, K]) as rows that the kernels can read (unit last stride,
+    no overlap): (tensor, N, row stride, dtype code)."""
+    code = DTYPE_CODE.get(x.dtype)
+    if code is None:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    shape = x.shape
+    if len(shape) > 2 or len(shape) == 0 or shape[-1] != K:
+        raise ValueError(f"x must be [K={K}] or [N, K={K}], got {tuple(shape)}")
+    if len(shape) == 1:
+        return (x if x.stride(0) == 1 or K == 1 else x.contiguous()), 1, K, code
+    N = shape[0]
+    s0, s1 = x.stride()
+    if (s1 != 1 and K > 1) or (s0 < K and N > 1):
+        x, s0 = x.contiguous(), K
+    return x, N, s0, code
+
+
+def out_for(y, shape, dtype, device, vec: bool):
+    """The output rows [N, M] of a call: (tensor to return, row stride)."""
+    if y is None:
+        return torch.empty(shape[1:] if vec else shape, dtype=dtype, device=device), shape[1]
+    want = tuple(shape[1:] if vec else shape)
+    if y.dtype != dtype or y.device != device or tuple(y.shape) != want:
+        raise ValueError(f"y must be a {dtype} tensor {want} on {device}")
+    if (y.stride(-1) != 1 and shape[1] > 1) or (not vec and shape[0] > 1 and y.stride(0) < shape[1]):
+        raise ValueError("y must have unit last stride and rows that do not overlap")
+    return y, (shape[1] if vec else y.stride(0))
+
+
+def stream_of(stream, device) -> int:
+    return _raw_stream(device.index) if stream is None else stream
+
+
+# one per (device, stream), grown on demand: calls on one stream are ordered
+_WS: dict = {}
+
+
+def workspace(device, nbytes: int, stream):
+    """(tensor, pointer, bytes) of a call's workspace.  Under capture a buffer
+    of its own, from the graph's memory; for a raw stream handle none (the
+    library's own buffer of that stream), since torch's allocator would not
+    know that the stream uses it."""
+    if stream is not None:
+        return None, None, 0
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return ws, ws.data_ptr(), nbytes
+    key = (device.index, _raw_stream(device.index))
+    ws = _WS.get(key)
+    if ws is None or ws[2] < nbytes:
+        t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = _WS[key] = (t, t.data_ptr(), nbytes)
+    return ws

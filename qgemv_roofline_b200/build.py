@@ -17,8 +17,8 @@ REPO = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libqgemv_b200.so")
 SOURCES = ["capi.cu", "gemv_soa.cu", "gemv_aos.cu", "quant.cu", "roof.cu", "harness.cu", "gemv_tma.cu", "gemv_mma.cu",
-           "gemv_tc.cu", "static_ws.cu", "multi_gpu.cu", "moe.cu"]
-HEADERS = ["qgemv_common.cuh", "qgemv_internal.h", "gemv_core.cuh"]
+           "gemv_tc.cu", "static_ws.cu", "multi_gpu.cu", "moe.cu", "int8.cu"]
+HEADERS = ["qgemv_common.cuh", "qgemv_internal.h", "gemv_core.cuh", "sm100.cuh"]
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -358,12 +358,14 @@ QGEMV_API int qgemv_soa_variant(int format, int variant, int32_t grid, const voi
 }
 
 QGEMV_API int qgemv_check_device_error(int clear, void* stream) {
-  int v = 0, w = 0, t = 0;
+  int v = 0, w = 0, t = 0, i = 0;
   if (int rc = read_device_error(clear, static_cast<cudaStream_t>(stream), &v)) return rc;
   if (int rc = read_mma_error(clear, static_cast<cudaStream_t>(stream), &w)) return rc;
   if (int rc = read_tc_error(clear, static_cast<cudaStream_t>(stream), &t)) return rc;
+  if (int rc = read_i8_error(clear, static_cast<cudaStream_t>(stream), &i)) return rc;
   if (!v) v = w;
   if (!v) v = t;
+  if (!v) v = i;
   if (v) return set_error(v, "a kernel reported %s on the device", qgemv_status_string(v));
   return OK;
 }
@@ -381,7 +383,8 @@ QGEMV_API int qgemv_set_wait_limit(int64_t microseconds) {
   }
   if (int rc = set_spin_limit(cycles)) return rc;
   if (int rc = set_mma_spin_limit(cycles)) return rc;
-  return set_tc_spin_limit(cycles);
+  if (int rc = set_tc_spin_limit(cycles)) return rc;
+  return set_i8_spin_limit(cycles);
 }
 
 QGEMV_API int32_t qgemv_tile_counters_used(int device) { return tile_counters_used(device); }
@@ -1001,6 +1004,115 @@ QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_r
   if (!router) return set_error(ERR_NULL, "router must not be NULL");
   return moe_entry(experts, router, x, dtype, ldx, nullptr, nullptr, 0, n_tokens, y, ldy,
                    workspace, workspace_bytes, stream);
+}
+
+namespace {
+int check_int8_rows(const char* what, const void* q, int64_t ld, int64_t rows, int64_t K) {
+  if (!q) return set_error(ERR_NULL, "%s must not be NULL", what);
+  if (misaligned(q, 16) || (rows > 1 && ld % 16))
+    return set_error(ERR_ALIGN, "%s and its rows must be 16-byte aligned", what);
+  if (rows > 1 && (ld < K || ld >= ((int64_t)1 << 39)))
+    return set_error(ERR_SHAPE, "%s: row stride %lld for %lld columns", what, (long long)ld, (long long)K);
+  return OK;
+}
+
+int check_int8_sizes(int64_t N, int64_t M, int64_t K) {
+  if (N < 0 || M < 0) return set_error(ERR_SHAPE, "negative shape N=%lld M=%lld", (long long)N, (long long)M);
+  if (K < 16 || K % 16) return set_error(ERR_SHAPE, "K=%lld is not a positive multiple of 16", (long long)K);
+  if (K > kInt8MaxK)
+    return set_error(ERR_UNSUPPORTED, "K=%lld: int32 sums are exact up to K=%lld", (long long)K,
+                     (long long)kInt8MaxK);
+  if (N >= kMaxDim || M >= kMaxDim - 128)
+    return set_error(ERR_UNSUPPORTED, "N and M must be below 2^31 (N=%lld M=%lld)", (long long)N, (long long)M);
+  return OK;
+}
+
+int int8_entry(const void* xq, const float* xs, int64_t ldx, const void* wq, const float* ws, int64_t ldw,
+               const float* bias, int64_t N, int64_t M, int64_t K, void* y, int ydt, int64_t ldy,
+               bool early_w, void* stream) {
+  if (ydt < 0 || ydt > 2) return set_error(ERR_ARG, "y_dtype must be 0, 1 or 2, got %d", ydt);
+  if (int rc = check_int8_sizes(N, M, K)) return rc;
+  if (N == 0 || M == 0) return OK;
+  if (int rc = check_int8_rows("xq", xq, ldx, N, K)) return rc;
+  if (int rc = check_int8_rows("wq", wq, ldw, M, K)) return rc;
+  if (!xs || !ws || !y) return set_error(ERR_NULL, "xs, ws and y must not be NULL");
+  if (misaligned(xs, 4) || misaligned(ws, 4) || misaligned(bias, 4) || misaligned(y, ydt == 0 ? 4 : 2))
+    return set_error(ERR_ALIGN, "scales and bias must be 4-byte aligned, y to its elements");
+  if (ldy < (N > 1 ? M : 0)) return set_error(ERR_SHAPE, "ldy=%lld < M=%lld", (long long)ldy, (long long)M);
+  Int8Call c;
+  c.xq = xq;
+  c.xs = xs;
+  c.ldx = N > 1 ? ldx : (K + 15) / 16 * 16;
+  c.wq = wq;
+  c.ws = ws;
+  c.ldw = M > 1 ? ldw : (K + 15) / 16 * 16;
+  c.bias = bias;
+  c.N = N;
+  c.M = M;
+  c.K = K;
+  c.y = y;
+  c.ldy = ldy;
+  c.ydt = ydt;
+  return int8_matmul(c, early_w, static_cast<cudaStream_t>(stream));
+}
+}  // namespace
+
+QGEMV_API int qgemv_int8_quantize(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K,
+                                  void* q, int64_t ldq, float* scales, void* stream) {
+  if (dtype < 0 || dtype > 2) return set_error(ERR_ARG, "dtype must be 0, 1 or 2, got %d", dtype);
+  if (rows < 0 || K < 1) return set_error(ERR_SHAPE, "rows=%lld K=%lld", (long long)rows, (long long)K);
+  if (rows >= kMaxDim || K >= kMaxDim - 16) return set_error(ERR_UNSUPPORTED, "rows and K must be below 2^31");
+  if (rows == 0) return OK;
+  if (!x || !q || !scales) return set_error(ERR_NULL, "x, q and scales must not be NULL");
+  if (misaligned(x, dtype == 0 ? 4 : 2) || misaligned(scales, 4))
+    return set_error(ERR_ALIGN, "x must be aligned to its elements, scales to 4 bytes");
+  if (rows > 1 && (ldx < K || ldq < K))
+    return set_error(ERR_SHAPE, "ldx=%lld and ldq=%lld must be at least K=%lld", (long long)ldx,
+                     (long long)ldq, (long long)K);
+  return int8_quantize(x, dtype, ldx, rows, K, q, ldq, K, scales, static_cast<cudaStream_t>(stream));
+}
+
+QGEMV_API int qgemv_int8_matmul(const void* xq, const float* xs, int64_t ldx, const void* wq,
+                                const float* ws, int64_t ldw, const float* bias, int64_t N,
+                                int64_t M, int64_t K, void* y, int y_dtype, int64_t ldy, void* stream) {
+  return int8_entry(xq, xs, ldx, wq, ws, ldw, bias, N, M, K, y, y_dtype, ldy, false, stream);
+}
+
+QGEMV_API size_t qgemv_int8_linear_workspace_bytes(int64_t N, int64_t K) {
+  if (N < 1 || K < 16 || K % 16 || K > kInt8MaxK || N >= kMaxDim) return 0;
+  return (size_t)((N + 31) / 32 * 32) * 4 + (size_t)N * K;
+}
+
+QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const void* wq, const float* ws,
+                                int64_t ldw, const float* bias, int64_t N, int64_t M, int64_t K,
+                                void* y, int y_dtype, int64_t ldy, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  if (dtype < 0 || dtype > 2) return set_error(ERR_ARG, "dtype must be 0, 1 or 2, got %d", dtype);
+  if (int rc = check_int8_sizes(N, M, K)) return rc;
+  if (N == 0 || M == 0) return OK;
+  if (!x) return set_error(ERR_NULL, "x must not be NULL");
+  if (misaligned(x, dtype == 0 ? 4 : 2)) return set_error(ERR_ALIGN, "x must be aligned to its elements");
+  if (ldx < (N > 1 ? K : 0)) return set_error(ERR_SHAPE, "ldx=%lld < K=%lld", (long long)ldx, (long long)K);
+  // everything the product checks, before anything is launched
+  if (y_dtype < 0 || y_dtype > 2) return set_error(ERR_ARG, "y_dtype must be 0, 1 or 2, got %d", y_dtype);
+  if (int rc = check_int8_rows("wq", wq, ldw, M, K)) return rc;
+  if (!ws || !y) return set_error(ERR_NULL, "ws and y must not be NULL");
+  if (misaligned(ws, 4) || misaligned(bias, 4) || misaligned(y, y_dtype == 0 ? 4 : 2))
+    return set_error(ERR_ALIGN, "scales and bias must be 4-byte aligned, y to its elements");
+  if (ldy < (N > 1 ? M : 0)) return set_error(ERR_SHAPE, "ldy=%lld < M=%lld", (long long)ldy, (long long)M);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t need = qgemv_int8_linear_workspace_bytes(N, K);
+  if (workspace) {
+    if (workspace_bytes < need)
+      return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
+    if (misaligned(workspace, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
+  } else if (int rc = stream_workspace(st, need, &workspace)) {
+    return rc;
+  }
+  float* xs = static_cast<float*>(workspace);
+  void* xq = static_cast<uint8_t*>(workspace) + (size_t)((N + 31) / 32 * 32) * 4;
+  if (int rc = int8_quantize(x, dtype, ldx, N, K, xq, K, K, xs, st)) return rc;
+  return int8_entry(xq, xs, K, wq, ws, ldw, bias, N, M, K, y, y_dtype, ldy, true, stream);
 }
 
 }  // extern "C"

@@ -62,6 +62,7 @@
 // and the CTA frees its TMEM before it returns.
 #include "qgemv_common.cuh"
 #include "qgemv_internal.h"
+#include "sm100.cuh"
 
 #include <algorithm>
 #include <cstring>
@@ -178,19 +179,6 @@ static_assert(TC_ABYTES % 1024 == 0 && TcFmt<4, 2>::WSTAGE % 1024 == 0 &&
 __device__ __forceinline__ long long tc_spin_limit() {
   return *(volatile long long*)&g_tc_spin_limit;
 }
-__device__ __forceinline__ uint32_t saddr(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
 // Bounded wait; gives up at once when another thread raised the abort flag.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try(bar, parity)) return true;
@@ -214,88 +202,6 @@ __device__ __forceinline__ void mbar_wait_drain(uint32_t bar, uint32_t parity) {
   while (!mbar_try(bar, parity) && clock64() - t0 < lim) {
   }
 }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major operand in the canonical
-// 128-byte-swizzled layout: start address >> 4 (bits 0-13), leading byte
-// offset 16 >> 4 (bits 16-29; not used by swizzled K-major operands), stride
-// byte offset 1024 >> 4 between 8-row groups (bits 32-45), descriptor version
-// 1 (bits 46-47), base offset 0 (atoms 1024-byte aligned), layout type 2 =
-// SWIZZLE_128B (bits 61-63).  Block b of a box starts 32 * b bytes into the
-// atom row: the hardware applies the swizzle to the computed addresses.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) |
-         ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
-}
-
-// 2-D tiled tensor copy global -> shared (no multicast); c0 is the inner
-// coordinate in elements (its byte offset a multiple of 16), c1 the row.
-__device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap* map, int c0, int c1,
-                                           uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
-}
-
-// 32 lanes x NC consecutive 32-bit TMEM columns.
-template <int NC>
-__device__ __forceinline__ void tmem_ld(uint32_t ta, uint32_t (&v)[NC]) {
-  if constexpr (NC == 1) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v[0]) : "r"(ta));
-  } else if constexpr (NC == 2) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];"
-                 : "=r"(v[0]), "=r"(v[1])
-                 : "r"(ta));
-  } else if constexpr (NC == 4) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(ta));
-  } else if constexpr (NC == 8) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
-                   "=r"(v[6]), "=r"(v[7])
-                 : "r"(ta));
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-          "=r"(v[14]), "=r"(v[15])
-        : "r"(ta));
-  }
-}
-
 struct TcArgs {
   // SoA planes (soa != 0): quants [M][K or K/2] bytes in boxes of 128 bytes x
   // 128 rows, 128-byte swizzle (exactly the MMA's A layout for q8_0); scales

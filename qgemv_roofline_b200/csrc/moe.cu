@@ -51,6 +51,7 @@
 
 #include "qgemv_common.cuh"
 #include "qgemv_internal.h"
+#include "sm100.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -84,11 +85,6 @@ __device__ __forceinline__ float load_as_f32(const void* p, int dt, int64_t i) {
   if (dt == 0) return static_cast<const float*>(p)[i];
   if (dt == 1) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
   return to_f32(static_cast<const __half*>(p)[i]);
-}
-
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_trigger() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ---------------------------------------------------------- fixed point
@@ -529,9 +525,6 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
 }
 
 // ------------------------------------------------------- streaming products
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -751,7 +744,7 @@ __global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_up(MoeArgs a) {
   const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F);
   const int units = tb.nent * fc;
   const int64_t tile = (int64_t)kg * GB;  // one 16-row tile
-  Ring<FMT> ring{smem_addr(up_smem) + (uint32_t)(warp * D * GB), 0, 0};
+  Ring<FMT> ring{saddr(up_smem) + (uint32_t)(warp * D * GB), 0, 0};
   // the tile of unit u that this warp reads: expert, then 8-row pairs
   auto src_of = [&](int u) {
     const uint32_t en = tb.ent[u / fc];
@@ -837,7 +830,7 @@ __global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_down(MoeArgs a, int ydt) 
   const int rt = blockIdx.x / cs * MOE_W + warp, nrt = a.K / 16;  // this warp's 16 rows
   const bool live = rt < nrt;
   const int64_t tile = (int64_t)fg * GB;
-  Ring<FMT> ring{smem_addr(dn_smem) + (uint32_t)(warp * D * GB), 0, 0};
+  Ring<FMT> ring{saddr(dn_smem) + (uint32_t)(warp * D * GB), 0, 0};
   auto src_of = [&](int en) {
     return a.down + ((int64_t)(tb.ent[en] & 1023u) * nrt + rt) * tile;
   };

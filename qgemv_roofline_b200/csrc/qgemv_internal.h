@@ -199,4 +199,27 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
                 const int* ids, const float* weights, int slots, int64_t N, void* y, int64_t ldy,
                 void* ws, cudaStream_t st);
 
+// int8 products (int8.cu).  dtypes as above.
+constexpr int64_t kInt8MaxK = ((int64_t)1 << 17) - 1;  // K * 128 * 128 stays in int32
+struct Int8Call {
+  const void* xq = nullptr;  // int8 [N][ldx]
+  const float* xs = nullptr;
+  int64_t ldx = 0;
+  const void* wq = nullptr;  // int8 [M][ldw]
+  const float* ws = nullptr;
+  int64_t ldw = 0;
+  const float* bias = nullptr;
+  int64_t N = 0, M = 0, K = 0;
+  void* y = nullptr;
+  int64_t ldy = 0;
+  int ydt = 0;
+};
+int int8_quantize(const void* x, int xdt, int64_t ldx, int64_t N, int64_t K, void* q, int64_t ldq,
+                  int64_t kpad, float* s, cudaStream_t st);
+// early_w: the launch before this one was int8_quantize's on the same stream
+// (the weights may be read before it has finished).
+int int8_matmul(const Int8Call& c, bool early_w, cudaStream_t st);
+int set_i8_spin_limit(long long cycles);
+int read_i8_error(int clear, cudaStream_t st, int* out);
+
 }  // namespace qg

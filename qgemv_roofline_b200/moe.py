@@ -20,42 +20,12 @@ import functools
 import torch
 
 from . import _lib
-from .gemv import QuantizedMatrix, _workspace
+from ._tensors import DTYPE_CODE, on_device_of_x, out_for, rows_of, stream_of, workspace
+from .gemv import QuantizedMatrix
 from .qformats import BLOCK_BYTES, QK
 
-DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 SCORING = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS, MAX_CHOICES = 1024, 32
-
-
-def _on_device_of_x(fn):
-    """Runs ``fn(x, ...)`` with the device of ``x`` current."""
-    @functools.wraps(fn)
-    def wrapper(x, *args, **kwargs):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            raise ValueError("x must be a CUDA tensor")
-        if x.get_device() == torch.cuda.current_device():
-            return fn(x, *args, **kwargs)
-        with torch.cuda.device(x.device):
-            return fn(x, *args, **kwargs)
-    return wrapper
-
-
-def _rows(x: torch.Tensor, K: int):
-    """x as [N, K] with unit last stride, and its dtype code."""
-    code = DTYPE_CODE.get(x.dtype)
-    if code is None:
-        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    X = x.unsqueeze(0) if x.dim() == 1 else x
-    if X.dim() != 2 or X.shape[1] != K:
-        raise ValueError(f"x must be [K={K}] or [N, K={K}], got {tuple(x.shape)}")
-    if X.stride(1) != 1 or (X.stride(0) < K and X.shape[0] > 1):
-        X = X.contiguous()  # the kernels read rows that do not overlap
-    return X, code
-
-
-def _stream(stream, device):
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
 
 
 def _router(router, top_k, scoring, bias, scale, normalize, device) -> _lib.MoeRouter:
@@ -76,7 +46,7 @@ def _router(router, top_k, scoring, bias, scale, normalize, device) -> _lib.MoeR
                           bool(normalize), scale)
 
 
-@_on_device_of_x
+@on_device_of_x
 def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, scoring: str = "softmax",
               bias: torch.Tensor | None = None, scale: float = 1.0, normalize: bool = True,
               stream: int | None = None):
@@ -89,14 +59,15 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, scoring: str
     the weights.  Returns ``(ids int32, weights float32)``, each [N, top_k] ([top_k] for a
     vector x), in descending order of score.
     """
-    X, code = _rows(x, router.shape[-1])
-    r = _router(router, top_k, scoring, bias, scale, normalize, x.device)
-    N = X.shape[0]
-    ids = torch.empty((N, top_k), dtype=torch.int32, device=x.device)
-    weights = torch.empty((N, top_k), dtype=torch.float32, device=x.device)
-    _lib.call("qgemv_moe_route", ctypes.byref(r), X.data_ptr(), code, X.stride(0), N, X.shape[1],
-              ids.data_ptr(), weights.data_ptr(), _stream(stream, x.device))
-    return (ids[0], weights[0]) if x.dim() == 1 else (ids, weights)
+    X, N, ldx, code = rows_of(x, router.shape[-1])
+    device = x.device
+    r = _router(router, top_k, scoring, bias, scale, normalize, device)
+    shape = (N, top_k) if x.dim() == 2 else (top_k,)
+    ids = torch.empty(shape, dtype=torch.int32, device=device)
+    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    _lib.call("qgemv_moe_route", ctypes.byref(r), X.data_ptr(), code, ldx, N, X.shape[-1],
+              ids.data_ptr(), weights.data_ptr(), stream_of(stream, device))
+    return ids, weights
 
 
 class QuantizedExperts:
@@ -128,6 +99,7 @@ class QuantizedExperts:
         with torch.cuda.device(dev):
             self.gate_up = self._tile(fmt, gate, up, E, F, K)
             self.down = self._tile(fmt_down, down, None, E, K, F)
+        self.device = dev
         self._set = _lib.ExpertSet(_lib.FORMAT_CODE[fmt], _lib.FORMAT_CODE[fmt_down], E, n_shared,
                                    K, F, self.gate_up.data_ptr(), self.down.data_ptr())
         self._ref = ctypes.byref(self._set)
@@ -183,40 +155,17 @@ class QuantizedExperts:
         return cls(planes(gate), planes(up), planes(down), n_shared)
 
     @property
-    def device(self):
-        return self.gate_up.device
-
-    @property
     def nbytes(self) -> int:
         """Bytes of the quantized weights (the tiles pad columns to 128)."""
         n = self.n_experts * self.hidden * self.ffn // QK
         return n * (2 * BLOCK_BYTES[self.fmt] + BLOCK_BYTES[self.fmt_down])
 
 
-def _out(y, X, x):
-    if y is None:
-        Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-        return Y, (Y[0] if x.dim() == 1 else Y)
-    if y.dtype != x.dtype or y.device != x.device:
-        raise ValueError("y must have the type and device of x")
-    Y = y.unsqueeze(0) if y.dim() == 1 else y
-    if Y.shape != X.shape or Y.stride(1) != 1 or (Y.shape[0] > 1 and Y.stride(0) < Y.shape[1]):
-        raise ValueError(f"y must be {tuple(x.shape)} with unit last stride")
-    return Y, y
-
-
 def _experts_on(experts, x):
-    if experts.device != x.device:
-        raise ValueError(f"the experts are on {experts.device}, x on {x.device}")
-
-
-def _ws(device, nbytes, stream):
-    """(pointer, bytes) of the workspace; for a raw stream handle none: torch's
-    allocator does not know that stream, so the library's own per-stream buffer."""
-    if stream is not None:
-        return None, 0
-    ws = _workspace(device, nbytes, None)
-    return ws.data_ptr(), ws.numel()
+    device = x.device
+    if experts.device != device:
+        raise ValueError(f"the experts are on {experts.device}, x on {device}")
+    return device
 
 
 @functools.lru_cache(maxsize=256)
@@ -224,7 +173,7 @@ def _ws_bytes(N, slots, hidden, ffn):
     return _lib.lib().qgemv_moe_workspace_bytes(N, slots, hidden, ffn)
 
 
-@_on_device_of_x
+@on_device_of_x
 def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
                 experts: QuantizedExperts, y: torch.Tensor | None = None,
                 stream: int | None = None) -> torch.Tensor:
@@ -234,50 +183,46 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     [0, E), -1 for instance, selects no expert; one that a token names twice counts with
     the sum of its weights; a token without experts gets zeros.
     """
-    _experts_on(experts, x)
-    X, code = _rows(x, experts.hidden)
-    Y, y = _out(y, X, x)
-    N = X.shape[0]
-    I, W = (ids.unsqueeze(0), weights.unsqueeze(0)) if ids.dim() == 1 else (ids, weights)
-    if (I.dim() != 2 or I.shape[0] != N or I.shape != W.shape or I.dtype != torch.int32
-            or W.dtype != torch.float32 or I.device != x.device or W.device != x.device
-            or not I.is_contiguous() or not W.is_contiguous()):
-        raise ValueError(f"ids (int32) and weights (float32) must be contiguous [N={N}, slots] on {x.device}")
-    slots = I.shape[1]
+    device = _experts_on(experts, x)
+    X, N, ldx, code = rows_of(x, experts.hidden)
+    vec = x.dim() == 1
+    slots = ids.shape[-1] if ids.dim() else 0
+    want = (slots,) if vec else (N, slots)
+    if (ids.shape != want or weights.shape != want or ids.dtype != torch.int32
+            or weights.dtype != torch.float32 or ids.device != device or weights.device != device
+            or not ids.is_contiguous() or not weights.is_contiguous()):
+        raise ValueError(f"ids (int32) and weights (float32) must be contiguous [N={N}, slots] on {device}")
     if not 1 <= slots <= MAX_CHOICES:
         raise ValueError(f"1 to {MAX_CHOICES} choices per token, got {slots}")
+    y, ldy = out_for(y, (N, experts.hidden), x.dtype, device, vec)
     if N == 0:
         return y
-    nbytes = _ws_bytes(min(N, 64), slots, experts.hidden, experts.ffn)
-    ws, nbytes = _ws(x.device, nbytes, stream)
-    _lib.call("qgemv_moe_experts", experts._ref, X.data_ptr(), code, X.stride(0), I.data_ptr(),
-              W.data_ptr(), slots, N, Y.data_ptr(), Y.stride(0), ws, nbytes,
-              _stream(stream, x.device))
+    _, ptr, nbytes = workspace(device, _ws_bytes(min(N, 64), slots, experts.hidden, experts.ffn), stream)
+    _lib.call("qgemv_moe_experts", experts._ref, X.data_ptr(), code, ldx, ids.data_ptr(),
+              weights.data_ptr(), slots, N, y.data_ptr(), ldy, ptr, nbytes, stream_of(stream, device))
     return y
 
 
-@_on_device_of_x
+@on_device_of_x
 def moe_layer(x: torch.Tensor, router: torch.Tensor, experts: QuantizedExperts, top_k: int, *,
               scoring: str = "softmax", bias: torch.Tensor | None = None, scale: float = 1.0,
               normalize: bool = True, y: torch.Tensor | None = None,
               stream: int | None = None) -> torch.Tensor:
     """A whole mixture-of-experts layer: ``moe_route`` over the experts that are not
     shared, then ``moe_experts`` with these and the shared ones (weight 1)."""
-    _experts_on(experts, x)
-    X, code = _rows(x, experts.hidden)
-    if tuple(router.shape) != (experts.n_experts - experts.n_shared, experts.hidden):
+    device = _experts_on(experts, x)
+    X, N, ldx, code = rows_of(x, experts.hidden)
+    if router.shape != (experts.n_experts - experts.n_shared, experts.hidden):
         raise ValueError(f"router must be [{experts.n_experts - experts.n_shared}, {experts.hidden}], "
                          f"got {tuple(router.shape)}")
-    r = _router(router, top_k, scoring, bias, scale, normalize, x.device)
+    r = _router(router, top_k, scoring, bias, scale, normalize, device)
     slots = top_k + experts.n_shared
     if slots > MAX_CHOICES:
         raise ValueError(f"{slots} choices per token (shared experts included), at most {MAX_CHOICES}")
-    Y, y = _out(y, X, x)
-    N = X.shape[0]
+    y, ldy = out_for(y, (N, experts.hidden), x.dtype, device, x.dim() == 1)
     if N == 0:
         return y
-    nbytes = _ws_bytes(min(N, 64), slots, experts.hidden, experts.ffn)
-    ws, nbytes = _ws(x.device, nbytes, stream)
-    _lib.call("qgemv_moe_layer", experts._ref, ctypes.byref(r), X.data_ptr(), code, X.stride(0), N,
-              Y.data_ptr(), Y.stride(0), ws, nbytes, _stream(stream, x.device))
+    _, ptr, nbytes = workspace(device, _ws_bytes(min(N, 64), slots, experts.hidden, experts.ffn), stream)
+    _lib.call("qgemv_moe_layer", experts._ref, ctypes.byref(r), X.data_ptr(), code, ldx, N,
+              y.data_ptr(), ldy, ptr, nbytes, stream_of(stream, device))
     return y

@@ -212,3 +212,35 @@ def test_moe_validation():
     assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 32, 160) == 3 * 2 * 2 * (1024 + 128)
     assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 40, 160) == 0
     assert _lib.lib().qgemv_moe_workspace_bytes(1, 33, 64, 64) == 0
+
+
+def test_int8_validation():
+    E = _lib
+
+    def mm(xq=FAKE, xs=FAKE, ldx=64, wq=FAKE, ws=FAKE, ldw=64, b=None, n=2, m=8, k=64, y=FAKE, dt=0, ldy=8):
+        return rc("qgemv_int8_matmul", xq, xs, ldx, wq, ws, ldw, b, n, m, k, y, dt, ldy, None)
+
+    assert mm(n=0) == 0 and mm(m=0, ldy=0) == 0
+    assert mm(n=-1) == 2 and mm(m=-1) == 2 and mm(k=0) == 2 and mm(k=40) == 2
+    assert mm(k=1 << 17, ldx=1 << 17, ldw=1 << 17) == 5 and "int32" in E.last_error()
+    assert mm(n=1 << 31) == 5 and mm(m=1 << 31) == 5
+    assert mm(xq=None) == 1 and mm(xs=None) == 1 and mm(wq=None) == 1 and mm(ws=None) == 1 and mm(y=None) == 1
+    assert mm(xq=FAKE + 8) == 3 and mm(wq=FAKE + 4) == 3 and mm(ldx=72) == 3 and mm(ldw=65) == 3
+    assert mm(xs=FAKE + 2) == 3 and mm(b=FAKE + 1) == 3 and mm(y=FAKE + 2) == 3
+    assert mm(ldx=48) == 2 and mm(ldw=32) == 2 and mm(ldy=7) == 2 and mm(dt=3) == 7
+
+    def lin(x=FAKE, dt=0, ldx=64, wq=FAKE, n=2, k=64, y=FAKE, ydt=0, ws=FAKE, nb=1 << 20):
+        return rc("qgemv_int8_linear", x, dt, ldx, wq, FAKE, 64, None, n, 8, k, y, ydt, 8, ws, nb, None)
+
+    assert lin(n=0) == 0 and lin(x=None) == 1 and lin(dt=-1) == 7 and lin(ydt=9) == 7
+    assert lin(x=FAKE + 2) == 3 and lin(ldx=63) == 2 and lin(k=72) == 2 and lin(y=None) == 1
+    assert lin(ws=FAKE + 4) == 3 and lin(nb=100) == 7 and "workspace" in E.last_error()
+    assert _lib.lib().qgemv_int8_linear_workspace_bytes(33, 64) == 64 * 4 + 33 * 64
+    assert _lib.lib().qgemv_int8_linear_workspace_bytes(33, 65) == 0
+
+    def quant(x=FAKE, dt=0, ldx=64, n=2, k=64, q=FAKE, ldq=64, s=FAKE):
+        return rc("qgemv_int8_quantize", x, dt, ldx, n, k, q, ldq, s, None)
+
+    assert quant(n=0) == 0 and quant(n=-1) == 2 and quant(k=0) == 2 and quant(dt=4) == 7
+    assert quant(x=None) == 1 and quant(q=None) == 1 and quant(s=None) == 1
+    assert quant(ldx=63) == 2 and quant(ldq=63) == 2 and quant(s=FAKE + 2) == 3 and quant(x=FAKE + 1, dt=1) == 3
