@@ -358,14 +358,16 @@ QGEMV_API int qgemv_soa_variant(int format, int variant, int32_t grid, const voi
 }
 
 QGEMV_API int qgemv_check_device_error(int clear, void* stream) {
-  int v = 0, w = 0, t = 0, i = 0;
+  int v = 0, w = 0, t = 0, i = 0, m = 0;
   if (int rc = read_device_error(clear, static_cast<cudaStream_t>(stream), &v)) return rc;
   if (int rc = read_mma_error(clear, static_cast<cudaStream_t>(stream), &w)) return rc;
   if (int rc = read_tc_error(clear, static_cast<cudaStream_t>(stream), &t)) return rc;
   if (int rc = read_i8_error(clear, static_cast<cudaStream_t>(stream), &i)) return rc;
+  if (int rc = read_moe_error(clear, static_cast<cudaStream_t>(stream), &m)) return rc;
   if (!v) v = w;
   if (!v) v = t;
   if (!v) v = i;
+  if (!v) v = m;
   if (v) return set_error(v, "a kernel reported %s on the device", qgemv_status_string(v));
   return OK;
 }
@@ -384,7 +386,8 @@ QGEMV_API int qgemv_set_wait_limit(int64_t microseconds) {
   if (int rc = set_spin_limit(cycles)) return rc;
   if (int rc = set_mma_spin_limit(cycles)) return rc;
   if (int rc = set_tc_spin_limit(cycles)) return rc;
-  return set_i8_spin_limit(cycles);
+  if (int rc = set_i8_spin_limit(cycles)) return rc;
+  return set_moe_spin_limit(cycles);
 }
 
 QGEMV_API int32_t qgemv_tile_counters_used(int device) { return tile_counters_used(device); }

@@ -23,17 +23,23 @@
 //    shared memory in rank order (deterministic).
 //
 // The arithmetic is the library's exact-integer scheme.  A block of 32
-// activations is rounded to integers X = rint(x FX / max |x|), FX = 0x7F7F7F
-// (a step of max |x| 2^-23; the GEMVs' powers of two leave 2^-22 to 2^-21, and
-// here two products follow one another: measured 7.5e-7 -> 2.9e-7 relative
-// error of y), and split into three signed byte digits
-// X = p0 + 2^8 p1 + 2^16 p2; the integer dots of the block's quants with the
-// digits are exact (mma.sync.m16n8k32.s8, |S| <= 32 * 128 * 128 = 2^19), and
-// each block is scaled once: acc += (S0 + 2^8 S1 + 2^16 S2) (d max / FX).  With one or two
-// tokens the three digits of both are the 8 columns of ONE MMA; with more,
-// each digit plane has an MMA of 8 tokens.  The MMA's accumulator starts at
-// the bits of 1.5 * 2^23, so that its integer result read as a float is
-// 1.5 * 2^23 + S exactly: one subtraction instead of an integer conversion.
+// activations is rounded to integers X = rint(x FX / max |x|) and split into
+// signed byte digits X = p0 + 2^8 p1 (+ 2^16 p2); the integer dots of the
+// block's quants with the digits are exact (mma.sync.m16n8k32.s8,
+// |S| <= 32 * 128 * 128 = 2^19), and each block is scaled once:
+// acc += (S0 + 2^8 S1 + 2^16 S2) (d max / FX).
+//
+//  * fp32 activations take three digits, FX = 0x7F7F7F (a step of max |x| 2^-23;
+//    the GEMVs' powers of two leave 2^-22 to 2^-21, and here two products
+//    follow one another: measured 7.5e-7 -> 2.9e-7 relative error of y);
+//  * bf16 and fp16 activations take two, FX = 0x7F7F: a step of max |x| 2^-15
+//    moves y by about 1e-5 of its size, a twentieth of fp16's own rounding of y
+//    (2^-12 on average) and a two-hundredth of bf16's, for x and for h.
+//
+// The 8 columns of an MMA are the digits of 4 tokens (two digits each) or 2
+// (three), so one MMA per block serves up to 4 or 2 tokens, and a lane's pair
+// of accumulators is one token's pair of digits, joined as integers
+// (|S0 + 2^8 S1| < 2^28) and converted once.
 // A block that holds a NaN or an infinity gets a NaN scale: y is NaN there.
 //
 // Weights are "expert tiles", laid out once: per expert, 16-row tiles; a
@@ -43,8 +49,11 @@
 // row + 8].  q4_0 nibbles are stored with bit 3 flipped: n ^ 8 shifted into
 // the high half of a byte is 16 (n - 8) as a signed byte, one or two
 // instructions; the 1/16 is folded into the activation scale (exact).  A warp
-// reads its tile as one contiguous stream through a private cp.async ring.
+// reads its tile as one contiguous stream through a private ring of bulk copies.
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -57,21 +66,34 @@ namespace cg = cooperative_groups;
 
 namespace qg {
 
+__device__ int g_moe_error = 0;
+__device__ long long g_moe_spin_limit = kDefaultSpinLimit;
+
 namespace {
 
 constexpr int MOE_NT = kMoeTokens;  // tokens per pass
-constexpr int MOE_W = 4;            // warps per CTA of the expert kernels
+constexpr int MOE_W = 4;            // row tiles (of 16) that a CTA's warps take side by side
+constexpr int MOE_UPK = 4;          // gate / up: warps that split a row tile's columns
+constexpr int MOE_DOWN_CL = 8;      // down: CTAs of a cluster, at most
+constexpr int UP_THREADS = 32 * MOE_W * MOE_UPK;
 constexpr int MOE_GCOLS = 128;      // columns of a group (4 blocks)
-constexpr int MOE_DIG = 384;        // digit bytes of a group: [3 planes][4 lanes][32]
-constexpr int MOE_ENT = 16;         // tokens of one entry, at most
-constexpr float MOE_MAGIC = 12582912.0f;  // 1.5 * 2^23
-constexpr uint32_t MOE_MAGIC_BITS = 0x4B400000u;
+// digit bytes of a group: [digits][4 lanes][32]
+template <int DIG> __host__ __device__ constexpr int dig_bytes() { return DIG * 128; }
+// tokens that share one MMA, and of one entry (one or two MMAs) at most: four
+// MMAs an entry do not fit the registers (they spilled 1 KB and cost all
+// calls 1.5x); an expert with more tokens streams its weights again, from L2
+template <int DIG> __host__ __device__ constexpr int tok_mma() { return DIG == 2 ? 4 : 2; }
+template <int DIG> __host__ __device__ constexpr int ent_tok() { return 2 * tok_mma<DIG>(); }
 
 // bytes of a group (16 rows x 128 columns): quants, then 64 fp16 scales
 template <int FMT> __host__ __device__ constexpr int grp_q() { return FMT == 8 ? 2048 : 1024; }
 template <int FMT> __host__ __device__ constexpr int grp_bytes() { return grp_q<FMT>() + 128; }
-// ring slots per warp: about 11 KB either way, 44 KB per CTA, 4 CTAs per SM
-template <int FMT> __host__ __device__ constexpr int ring_depth() { return FMT == 8 ? 5 : 10; }
+// Ring of a warp: two slots of 2 (q8_0) or 4 (q4_0) groups, 9 KB either way,
+// 144 KB on an SM of 16 warps
+constexpr int MOE_RING = 2;
+template <int FMT> __host__ __device__ constexpr int slot_groups() { return FMT == 8 ? 2 : 4; }
+template <int FMT> __host__ __device__ constexpr int slot_bytes() { return slot_groups<FMT>() * grp_bytes<FMT>(); }
+template <int FMT> __host__ __device__ constexpr int ring_bytes() { return MOE_RING * slot_bytes<FMT>(); }
 
 __host__ __device__ constexpr int groups_of(int64_t cols) {
   return (int)((cols + MOE_GCOLS - 1) / MOE_GCOLS);
@@ -95,8 +117,11 @@ struct BlockScale {
   float s;      // FX / (max up); 0 for an all-zero or non-finite block (X = 0)
   float scale;  // max / FX; 0 for an all-zero block, NaN for a non-finite one
 };
-constexpr float MOE_FX = 8355711.0f;  // 0x7F7F7F: three signed byte digits of 127
+// 0x7F7F7F or 0x7F7F: every signed byte digit at most 127
+template <int DIG> __host__ __device__ constexpr int fx_max() { return DIG == 2 ? 0x7F7F : 0x7F7F7F; }
+template <int DIG>
 __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
+  constexpr float FX = (float)fx_max<DIG>();
   BlockScale b{1.0f, 0.0f, 0.0f};
   const float m = __uint_as_float(amax);
   if (amax >= 0x7F800000u) {
@@ -104,17 +129,19 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
   } else if (amax != 0u) {
     const bool tiny = m < 5.421010862427522e-20f;  // 2^-64
     b.up = tiny ? 18446744073709551616.0f : 1.0f;
-    b.s = MOE_FX / (m * b.up);
-    b.scale = m * b.up / MOE_FX * (tiny ? 5.421010862427522e-20f : 1.0f);
+    b.s = FX / (m * b.up);
+    b.scale = m * b.up / FX * (tiny ? 5.421010862427522e-20f : 1.0f);
   }
   return b;
 }
-// X + 0x808080 of one value: byte p, with its top bit flipped, is digit p.
-// |X| <= 0x7F7F7F also where the product rounds up (the clamp), so the biased
-// value keeps to 24 bits.  A value of a non-finite block gives 0.
+// X + 0x808080 (or 0x8080) of one value: byte p, with its top bit flipped, is
+// digit p.  The clamp holds |X| <= FX also where the product rounds up, so the
+// biased value keeps to its digits.  A value of a non-finite block gives 0.
+template <int DIG>
 __device__ __forceinline__ uint32_t fixed_biased(float v, const BlockScale& b) {
+  constexpr int FX = fx_max<DIG>();
   const int X = b.s == 0.0f ? 0 : __float2int_rn(v * b.up * b.s);
-  return (uint32_t)(min(max(X, -0x7F7F7F), 0x7F7F7F) + 0x808080);
+  return (uint32_t)(min(max(X, -FX), FX) + (DIG == 2 ? 0x8080 : 0x808080));
 }
 
 struct MoeArgs {
@@ -122,9 +149,9 @@ struct MoeArgs {
   const void* x;
   int64_t ldx;
   int xdt;
-  uint8_t* xdig;   // [N][K groups][384]
+  uint8_t* xdig;   // [N][K groups][digit bytes]
   float* xs;       // [N][K groups * 4]
-  uint8_t* hdig;   // [N * slots][F groups][384]
+  uint8_t* hdig;   // [N * slots][F groups][digit bytes]
   float* hs;       // [N * slots][F groups * 4]
   // choices
   const int* ids;        // [N][slots]
@@ -149,13 +176,14 @@ struct RouteArgs {
   float scale;
   int* ids;        // [N][k + shared]
   float* weights;
-  int clusters;    // CTAs [0, 8 * clusters) route; the others prepare x
+  int clusters;    // CTAs [0, cluster size * clusters) route; the others prepare x
 };
 
 // Fixed-point form of x, one warp per (token, group of 128 columns); columns
 // past K get zero digits and a zero scale.  Also the zero scales of h's blocks
 // past F (their digits are never read into a nonzero product, but a stale NaN
 // scale would be).
+template <int DIG>
 __device__ void prepare_x(const MoeArgs& a, int warp, int nwarps, int lane) {
   const int kg = groups_of(a.K), fg = groups_of(a.F), fb = a.F / QK;
   for (int i = warp; i < a.N * kg; i += nwarps) {
@@ -170,16 +198,16 @@ __device__ void prepare_x(const MoeArgs& a, int warp, int nwarps, int lane) {
     for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const BlockScale b = block_scale(m);
+    const BlockScale b = block_scale<DIG>(m);
     uint32_t f[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = fixed_biased(v[j], b);
+    for (int j = 0; j < 4; ++j) f[j] = fixed_biased<DIG>(v[j], b);
     // lane 8 blk + j holds elements 4j ... of block blk: B fragment register
     // j / 4 of MMA lane j % 4
     const int blk = lane >> 3, t = lane & 3, half = (lane >> 2) & 1;
-    uint8_t* dst = a.xdig + (int64_t)i * MOE_DIG + t * 32 + blk * 8 + half * 4;
+    uint8_t* dst = a.xdig + (int64_t)i * dig_bytes<DIG>() + t * 32 + blk * 8 + half * 4;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < DIG; ++p) {
       const uint32_t w = ((f[0] >> (8 * p)) & 0xFFu) | (((f[1] >> (8 * p)) & 0xFFu) << 8) |
                          (((f[2] >> (8 * p)) & 0xFFu) << 16) | (((f[3] >> (8 * p)) & 0xFFu) << 24);
       *reinterpret_cast<uint32_t*>(dst + p * 128) = w ^ 0x80808080u;
@@ -194,10 +222,12 @@ __device__ void prepare_x(const MoeArgs& a, int warp, int nwarps, int lane) {
 // ------------------------------------------------------------- routing
 constexpr int RT_THREADS = 256;
 constexpr int RT_WARPS = RT_THREADS / 32;
-constexpr int RT_CL = 8;    // CTAs of a routing cluster
+// CTAs of a routing cluster that takes TN tokens (16 is the opt-in size; a
+// single token's logits are all latency, so they are spread widest)
+template <int TN> __host__ __device__ constexpr int rt_cl() { return TN == 1 ? 16 : 8; }
 constexpr int RT_TE = 4;    // experts of a warp's tile
 // x columns staged at a time, as doubles (32 KB)
-template <int TN> __host__ __device__ constexpr int rt_chunk() { return TN == 1 ? 4096 : 512; }
+template <int TN> __host__ __device__ constexpr int rt_chunk() { return TN == 1 ? 4096 : TN == 2 ? 2048 : 512; }
 
 // Ordering key of a score: larger key = larger score; NaN lowest; +0 == -0.
 __device__ __forceinline__ unsigned long long rank_key(double v) {
@@ -317,8 +347,8 @@ __device__ void route_token(const RouteArgs& r, const float* logit, unsigned lon
   }
 }
 
-// CTAs [0, 8 * clusters): cluster c routes tokens [TN c, TN c + TN), CTA rank
-// r computing the logits of experts [E r / 8, E (r + 1) / 8) and choosing for
+// CTAs [0, CL * clusters): cluster c routes tokens [TN c, TN c + TN), CTA rank
+// r computing the logits of experts [E r / CL, E (r + 1) / CL) and choosing for
 // token TN c + r.  A warp takes tiles of 4 experts x TN tokens; with fewer
 // tiles than warps the columns are split over them too.  The sums are in
 // fp64 (measured here: 64 FMA per clock and SM, the conversions from fp32 a
@@ -328,10 +358,13 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
   extern __shared__ __align__(16) uint8_t rt_smem[];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int RT_CL = rt_cl<TN>();
   if ((int)blockIdx.x >= RT_CL * r.clusters) {
     pdl_wait();
-    prepare_x(a, (blockIdx.x - RT_CL * r.clusters) * RT_WARPS + warp,
-              (gridDim.x - RT_CL * r.clusters) * RT_WARPS, lane);
+    const int w = (blockIdx.x - RT_CL * r.clusters) * RT_WARPS + warp;
+    const int nw = (gridDim.x - RT_CL * r.clusters) * RT_WARPS;
+    if (a.xdt == 0) prepare_x<3>(a, w, nw, lane);
+    else prepare_x<2>(a, w, nw, lane);
     return;
   }
   constexpr int CH = rt_chunk<TN>();
@@ -355,43 +388,62 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
   for (int t0 = 0; t0 < tiles; t0 += RT_WARPS / ks) {
     const int tl = t0 + warp / ks, eb = e0 + tl * RT_TE;
     double acc[RT_TE * TN] = {};
+    auto load = [&](float (&w)[RT_TE][4], int c) {
+#pragma unroll
+      for (int i = 0; i < RT_TE; ++i)
+        load4(w[i], r.w, r.wdt, (int64_t)min(eb + i, e1 - 1) * r.ldw + c + 4 * lane, K - c - 4 * lane, vec);
+    };
+    auto step = [&](const float (&w)[RT_TE][4], int cb) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        double wd[RT_TE][2];
+#pragma unroll
+        for (int i = 0; i < RT_TE; ++i) {
+          wd[i][0] = (double)w[i][2 * h];
+          wd[i][1] = (double)w[i][2 * h + 1];
+        }
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+          const double2 xv = *reinterpret_cast<const double2*>(xd + n * CH + cb + h * 64 + lane * 2);
+#pragma unroll
+          for (int i = 0; i < RT_TE; ++i) {
+            acc[i * TN + n] = fma(wd[i][0], xv.x, acc[i * TN + n]);
+            acc[i * TN + n] = fma(wd[i][1], xv.y, acc[i * TN + n]);
+          }
+        }
+      }
+    };
+    // the first two steps' weights are on their way while x is staged
+    constexpr int PRE = TN <= 2 ? 2 : 0;
+    float pre[PRE > 0 ? PRE : 1][RT_TE][4];
+    if (tl < tiles)
+#pragma unroll
+      for (int j = 0; j < PRE; ++j)
+        if ((sl + j * ks) * 128 < min(CH, K)) load(pre[j], (sl + j * ks) * 128);
     for (int c0 = 0; c0 < K; c0 += CH) {
       const int cn = min(CH, K - c0);
       __syncthreads();
       // column 128 i + 4 l + j sits at 128 i + 64 (j / 2) + 2 l + j % 2: a lane
       // reads its four columns with two conflict-free 16-byte loads
-      for (int i = threadIdx.x; i < TN * CH; i += RT_THREADS) {
-        const int n = i / CH, c = i % CH;
-        const double v = n < nn && c < cn ? load_as_f64(a.x, a.xdt, (int64_t)(n0 + n) * a.ldx + c0 + c) : 0.0;
-        xd[n * CH + (c & ~127) + ((c >> 1) & 1) * 64 + ((c >> 2) & 31) * 2 + (c & 1)] = v;
-      }
+      const int cr = (cn + 127) & ~127;
+      for (int n = 0; n < TN; ++n)
+        for (int c = threadIdx.x; c < cr; c += RT_THREADS) {
+          const double v = n < nn && c < cn ? load_as_f64(a.x, a.xdt, (int64_t)(n0 + n) * a.ldx + c0 + c) : 0.0;
+          xd[n * CH + (c & ~127) + ((c >> 1) & 1) * 64 + ((c >> 2) & 31) * 2 + (c & 1)] = v;
+        }
       __syncthreads();
       if (tl < tiles) {
+        int j = 0;
+        if (c0 == 0) {
+#pragma unroll
+          for (; j < PRE; ++j)
+            if ((sl + j * ks) * 128 < cn) step(pre[j], (sl + j * ks) * 128);
+        }
 #pragma unroll 2
-        for (int cb = sl * 128; cb < cn; cb += ks * 128) {
+        for (int cb = (sl + j * ks) * 128; cb < cn; cb += ks * 128) {
           float w[RT_TE][4];
-#pragma unroll
-          for (int i = 0; i < RT_TE; ++i)
-            load4(w[i], r.w, r.wdt, (int64_t)min(eb + i, e1 - 1) * r.ldw + c0 + cb + 4 * lane,
-                  cn - cb - 4 * lane, vec);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            double wd[RT_TE][2];
-#pragma unroll
-            for (int i = 0; i < RT_TE; ++i) {
-              wd[i][0] = (double)w[i][2 * h];
-              wd[i][1] = (double)w[i][2 * h + 1];
-            }
-#pragma unroll
-            for (int n = 0; n < TN; ++n) {
-              const double2 xv = *reinterpret_cast<const double2*>(xd + n * CH + cb + h * 64 + lane * 2);
-#pragma unroll
-              for (int i = 0; i < RT_TE; ++i) {
-                acc[i * TN + n] = fma(wd[i][0], xv.x, acc[i * TN + n]);
-                acc[i * TN + n] = fma(wd[i][1], xv.y, acc[i * TN + n]);
-              }
-            }
-          }
+          load(w, c0 + cb);
+          step(w, cb);
         }
       }
     }
@@ -427,8 +479,8 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
 }
 
 // --------------------------------------------------- entries of the experts
-// The chosen experts in ascending order, each with up to 16 of its tokens (an
-// expert with more has several entries), built by every CTA for itself from
+// The chosen experts in ascending order, each with up to MOE_ENT of its tokens
+// (an expert with more has several entries), built by every CTA for itself from
 // the choices.  A choice outside [0, E) selects nothing; an expert that one
 // token names twice counts once, with the sum of the weights.  An expert's
 // tokens are kept as a 64-bit mask and taken in ascending order: every CTA
@@ -436,18 +488,28 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
 struct Table {
   uint32_t* mask;   // [E][2] tokens of the expert
   int* first;       // [E]
-  uint32_t* ent;    // [max_ent] expert | first << 10 | count << 22
+  // [max_ent] expert | first << 10 | count << 22 | its place among the
+  // expert's entries << 26 (64 tokens in entries of 4: 15 at most)
+  uint32_t* ent;
   uint32_t* tmp;    // [P]
   uint32_t* sorted; // [P] choice | token << 16, by expert
   float* w;         // [P]
   int nent;
+  // entries of entry e's expert
+  __device__ __forceinline__ int run(int e) const {
+    const uint32_t x = ent[e] & 1023u;
+    const int c = __popc(mask[2 * x]) + __popc(mask[2 * x + 1]);
+    return (c + per_entry - 1) / per_entry;
+  }
+  int per_entry;
 };
 __host__ __device__ __forceinline__ size_t table_bytes(int E, int P, int max_ent) {
   return (size_t)(3 * E + max_ent + 3 * P) * 4;
 }
 
+template <int MOE_ENT>
 __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
-  __shared__ uint32_t wsum[MOE_W];
+  __shared__ uint32_t wsum[32];
   const int P = a.N * a.slots, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Table t;
   t.mask = reinterpret_cast<uint32_t*>(mem);
@@ -497,7 +559,7 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   if (lane == 31) wsum[warp] = inc;
   __syncthreads();
   uint32_t before = inc - sum, total = 0u;
-  for (int i = 0; i < MOE_W; ++i) {
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) {
     if (i < warp) before += wsum[i];
     total += wsum[i];
   }
@@ -505,7 +567,7 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   for (int i = b; i < e; ++i) {
     const uint32_t c = count(i);
     for (uint32_t j = 0; j < c; j += MOE_ENT)
-      t.ent[n0++] = (uint32_t)i | (c0 + j) << 10 | min((uint32_t)MOE_ENT, c - j) << 22;
+      t.ent[n0++] = (uint32_t)i | (c0 + j) << 10 | min((uint32_t)MOE_ENT, c - j) << 22 | j / MOE_ENT << 26;
     t.first[i] = (int)c0;
     c0 += c;
   }
@@ -521,17 +583,31 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   }
   __syncthreads();
   t.nent = (int)(total >> 16);
+  t.per_entry = MOE_ENT;
   return t;
 }
 
 // ------------------------------------------------------- streaming products
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ long long moe_spin_limit() {
+  return *(volatile long long*)&g_moe_spin_limit;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Bounded wait for a copy.  One that runs out is reported and the warp goes on
+// (its results are lost); `late` makes it wait again for what is in flight
+// before it ends.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64(), lim = moe_spin_limit();
+  while (!mbar_try(bar, parity)) {
+    if (clock64() - t0 > lim) {
+      atomicExch(&g_moe_error, (int)ERR_TIMEOUT);
+      return true;
+    }
+  }
+  return false;
+}
+__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64(), lim = max(moe_spin_limit(), kDefaultSpinLimit);
+  while (!mbar_try(bar, parity) && clock64() - t0 < lim) {
+  }
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -550,344 +626,404 @@ __device__ __forceinline__ uint4 ldg128(const void* p) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ void mma_s8(float (&f)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  uint32_t c[4];
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%10,%10,%10,%10};"
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
       : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(MOE_MAGIC_BITS));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(c[i]) - MOE_MAGIC;
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0), "r"(0), "r"(0),
+        "r"(0));
 }
 
-// One warp's ring over a contiguous stream of groups.
+// One warp's ring over a stream of groups, filled a whole ring ahead by bulk
+// copies.  The stream is a list of contiguous segments: `next(src, n)` gives
+// the next segment's first byte and its number of groups, false at the end.  A
+// slot never holds groups of two segments.
 template <int FMT>
 struct Ring {
-  uint32_t base;  // shared address of the warp's slots
-  int in, out;    // next slot to fill / to read
-  __device__ __forceinline__ void fill(const uint8_t* src, int lane) {
-    constexpr int GB = grp_bytes<FMT>();
-    const uint32_t dst = base + (uint32_t)(in * GB);
-#pragma unroll
-    for (int i = 0; i < grp_q<FMT>() / 512; ++i)
-      cp16(dst + i * 512 + lane * 16, src + i * 512 + lane * 16);
-    if (lane < 8) cp16(dst + grp_q<FMT>() + lane * 16, src + grp_q<FMT>() + lane * 16);
-    in = in + 1 == ring_depth<FMT>() ? 0 : in + 1;
+  uint32_t base, bar;   // shared addresses of the slots and their barriers
+  int asked, taken;     // slots so far
+  const uint8_t* src;   // next group
+  int left;             // groups left in the segment
+  bool late;
+  static constexpr int SG = slot_groups<FMT>(), GB = grp_bytes<FMT>(), SB = slot_bytes<FMT>();
+  __device__ __forceinline__ void init(uint32_t slots, uint32_t bars, int lane) {
+    base = slots;
+    bar = bars;
+    asked = taken = 0;
+    src = nullptr;
+    left = 0;
+    late = false;
+    if (lane == 0) {
+      for (int i = 0; i < MOE_RING; ++i) mbar_init(bar + 8 * i, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+  }
+  template <typename Next>
+  __device__ __forceinline__ void ask(int lane, Next next) {
+    if (left == 0 && !next(src, left)) left = -1;
+    if (left > 0) {
+      const int m = min(SG, left), s = asked % MOE_RING;
+      if (lane == 0) {
+        mbar_expect_tx(bar + 8 * s, (uint32_t)(m * GB));
+        bulk_g2s(base + s * SB, src, (uint32_t)(m * GB), bar + 8 * s);
+      }
+      src += m * GB;
+      left -= m;
+      ++asked;
+    }
+  }
+  // the address of the next slot in turn, once its copy has landed
+  __device__ __forceinline__ uint32_t wait() {
+    const int s = taken % MOE_RING;
+    const uint32_t parity = (uint32_t)(taken / MOE_RING) & 1u;
+    if (!mbar_try(bar + 8 * s, parity)) late |= wait_slow(bar + 8 * s, parity);
+    return base + s * SB;
+  }
+  __device__ __forceinline__ void finish() {
+    if (__any_sync(0xffffffffu, late))
+      for (int i = max(0, asked - MOE_RING); i < asked; ++i)
+        drain(bar + 8 * (i % MOE_RING), (uint32_t)(i / MOE_RING) & 1u);
   }
 };
 
-// A fragments of blocks 2 * pr and 2 * pr + 1 of the group at `st`.
+// A fragments (block i of the pair in a[i]) and scales (rows g and g + 8) of
+// blocks 2 p and 2 p + 1 of the group at `st`.
 template <int FMT>
-__device__ __forceinline__ void load_a(uint32_t (&a)[2][4], uint32_t st, int pr, int lane) {
-  if (FMT == 8) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 v = lds128(st + (2 * pr + i) * 512 + lane * 16);
-      a[i][0] = v.x;
-      a[i][1] = v.y;
-      a[i][2] = v.z;
-      a[i][3] = v.w;
-    }
-  } else {
-    // words: block 2 pr (row g, row g + 8), block 2 pr + 1 (row g, row g + 8)
-    const uint4 v = lds128(st + pr * 512 + lane * 16);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        a[i][h] = (w[2 * i + h] << 4) & 0xF0F0F0F0u;      // columns 4t ...
-        a[i][2 + h] = w[2 * i + h] & 0xF0F0F0F0u;         // columns 16 + 4t ...
-      }
-  }
-}
-
-// acc over the tokens of an entry: MODE 2 (one or two tokens, their digits the
-// 8 columns of one MMA; acc[0], acc[1]: rows g and g + 8, this lane's digit
-// pair), 8 (acc[0..1] row g, [2..3] row g + 8, tokens 2t and 2t + 1) or 16
-// (then tokens 8 + 2t and 9 + 2t in acc[4..7]).
-template <int MODE> __host__ __device__ constexpr int acc_n() { return MODE == 2 ? 2 : MODE / 2; }
-
-// What an entry's tokens look like to a lane.
-template <int FMT, int MODE>
-struct Cols {
-  const uint8_t* dig[MODE == 16 ? 2 : 1];  // this lane's digits (column lane / 4)
-  const float* s[MODE == 2 ? 1 : MODE == 8 ? 2 : 4];  // scales of the lane's columns
-  float f;  // MODE 2: weight of the lane's digit pair
-  // row(i): the activation row of the entry's i-th token
-  template <typename Row>
-  __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups,
-                                      int cnt, int lane, Row row) {
-    const int n = lane >> 2, t = lane & 3;
-    const int64_t ds = (int64_t)groups * MOE_DIG, ss = (int64_t)groups * 4;
-    constexpr float Q = FMT == 8 ? 1.0f : 0.0625f;  // q4_0 quants come as 16 (n - 8)
-    if (MODE == 2) {
-      dig[0] = digits + row(min(n >> 2, cnt - 1)) * ds + (n & 3) * 128 + t * 32;
-      s[0] = scales + row(min(t >> 1, cnt - 1)) * ss;
-      f = ((t & 1) ? 65536.0f : 1.0f) * Q;
-    } else {
-      f = Q;
-#pragma unroll
-      for (int h = 0; h < MODE / 8; ++h) {
-        dig[h] = digits + row(min(8 * h + n, cnt - 1)) * ds + t * 32;
-        s[2 * h] = scales + row(min(8 * h + 2 * t, cnt - 1)) * ss;
-        s[2 * h + 1] = scales + row(min(8 * h + 2 * t + 1, cnt - 1)) * ss;
-      }
-    }
-  }
-};
-
-// One group: digits and scales of the columns (L1 / L2), then the quants.
-template <int FMT, int MODE, typename Wait>
-__device__ __forceinline__ void group_product(float (&acc)[acc_n<MODE>()], const Cols<FMT, MODE>& c,
-                                              int grp, uint32_t st, int lane, Wait wait) {
-  const uint32_t dst = st + grp_q<FMT>() + (lane >> 2) * 16;
-  if constexpr (MODE == 2) {
-    uint4 b[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (((lane >> 2) & 3) != 3) {
-      b[0] = ldg128(c.dig[0] + grp * MOE_DIG);
-      b[1] = ldg128(c.dig[0] + grp * MOE_DIG + 16);
-    }
-    const uint4 sv = ldg128(c.s[0] + grp * 4);
-    wait();
-    const uint4 dv = lds128(dst);
-#pragma unroll
-    for (int pr = 0; pr < 2; ++pr) {
-      uint32_t a[2][4];
-      load_a<FMT>(a, st, pr, lane);
+struct Quants {
+  uint32_t a[2][4];
+  float2 d[2];
+  __device__ __forceinline__ void load(uint32_t st, int p, int lane) {
+    uint2 dv;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                 : "=r"(dv.x), "=r"(dv.y)
+                 : "r"(st + grp_q<FMT>() + (lane >> 2) * 16 + p * 8)
+                 : "memory");
+    d[0] = __half22float2(*reinterpret_cast<const __half2*>(&dv.x));
+    d[1] = __half22float2(*reinterpret_cast<const __half2*>(&dv.y));
+    if (FMT == 8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float v[4];
-        mma_s8(v, a[i], i ? b[pr].z : b[pr].x, i ? b[pr].w : b[pr].y);
-        const int k = 2 * pr + i;
-        const float sc = __uint_as_float(k == 0 ? sv.x : k == 1 ? sv.y : k == 2 ? sv.z : sv.w) * c.f;
-        const uint32_t dw = k == 0 ? dv.x : k == 1 ? dv.y : k == 2 ? dv.z : dv.w;
-        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dw));
-        acc[0] = fmaf(fmaf(v[1], 256.0f, v[0]), d.x * sc, acc[0]);
-        acc[1] = fmaf(fmaf(v[3], 256.0f, v[2]), d.y * sc, acc[1]);
+        const uint4 v = lds128(st + (2 * p + i) * 512 + lane * 16);
+        a[i][0] = v.x;
+        a[i][1] = v.y;
+        a[i][2] = v.z;
+        a[i][3] = v.w;
       }
-    }
-  } else {
+    } else {
+      // words: block 2 p (row g, row g + 8), block 2 p + 1 (row g, row g + 8)
+      const uint4 v = lds128(st + p * 512 + lane * 16);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int h = 0; h < MODE / 8; ++h) {
-      uint4 b[3][2];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        b[p][0] = ldg128(c.dig[h] + grp * MOE_DIG + p * 128);
-        b[p][1] = ldg128(c.dig[h] + grp * MOE_DIG + p * 128 + 16);
-      }
-      const uint4 s0 = ldg128(c.s[2 * h] + grp * 4), s1 = ldg128(c.s[2 * h + 1] + grp * 4);
-      if (h == 0) wait();
-      const uint4 dv = lds128(dst);
-#pragma unroll
-      for (int pr = 0; pr < 2; ++pr) {
-        uint32_t a[2][4];
-        load_a<FMT>(a, st, pr, lane);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float v0[4], v1[4], v2[4];
-          mma_s8(v0, a[i], i ? b[0][pr].z : b[0][pr].x, i ? b[0][pr].w : b[0][pr].y);
-          mma_s8(v1, a[i], i ? b[1][pr].z : b[1][pr].x, i ? b[1][pr].w : b[1][pr].y);
-          mma_s8(v2, a[i], i ? b[2][pr].z : b[2][pr].x, i ? b[2][pr].w : b[2][pr].y);
-          const int k = 2 * pr + i;
-          const float c0 = __uint_as_float(k == 0 ? s0.x : k == 1 ? s0.y : k == 2 ? s0.z : s0.w) * c.f;
-          const float c1 = __uint_as_float(k == 0 ? s1.x : k == 1 ? s1.y : k == 2 ? s1.z : s1.w) * c.f;
-          const uint32_t dw = k == 0 ? dv.x : k == 1 ? dv.y : k == 2 ? dv.z : dv.w;
-          const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&dw));
-          const float sc[4] = {d.x * c0, d.x * c1, d.y * c0, d.y * c1};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[4 * h + j] = fmaf(fmaf(v2[j], 65536.0f, fmaf(v1[j], 256.0f, v0[j])), sc[j],
-                                  acc[4 * h + j]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        a[i >> 1][i & 1] = (w[i] << 4) & 0xF0F0F0F0u;    // columns 4t ...
+        a[i >> 1][2 + (i & 1)] = w[i] & 0xF0F0F0F0u;     // columns 16 + 4t ...
       }
     }
   }
-}
+};
 
-// The digit pairs of MODE 2 live in neighbouring lanes: their sum.
-template <int MODE>
-__device__ __forceinline__ void join(float (&acc)[acc_n<MODE>()]) {
-  if constexpr (MODE == 2) {
-    acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);
-    acc[1] += __shfl_xor_sync(0xffffffffu, acc[1], 1);
+// The digits and block scales of one MMA's tokens for a group, as a lane
+// holds them: its column lane / 4 is token (lane / 4) / (8 / tokens), the
+// digit the rest; its accumulators belong to columns 2t and 2t + 1.
+struct Digits {
+  uint4 b[2];
+  uint4 s;
+};
+template <int DIG>
+struct Cols {
+  const uint8_t* dig;
+  const float* s;
+  // row(i): the activation row of the i-th of `cnt` tokens; the columns of
+  // absent tokens repeat the last one's.  g0: the first group.
+  template <typename Row>
+  __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups, int g0,
+                                      int cnt, int lane, Row row) {
+    const int n = lane >> 2, t = lane & 3;
+    // three digits: column 3 (and 7) is idle and reads digit 2 again; its
+    // accumulator is dropped
+    const int tok = DIG == 2 ? n >> 1 : n >> 2, d = DIG == 2 ? n & 1 : min(n & 3, 2);
+    dig = digits + (row(min(tok, cnt - 1)) * groups + g0) * dig_bytes<DIG>() + d * 128 + t * 32;
+    s = scales + (row(min(DIG == 2 ? t : t >> 1, cnt - 1)) * groups + g0) * 4;
+  }
+  // the digits of the next group in turn
+  __device__ __forceinline__ void load(Digits& f) {
+    f.b[0] = ldg128(dig);
+    f.b[1] = ldg128(dig + 16);
+    f.s = ldg128(s);
+    dig += dig_bytes<DIG>();
+    s += 4;
+  }
+};
+
+// acc[0], acc[1]: rows g and g + 8 of the lane's token (three digits: the even
+// lane holds the two low digits' sum, the odd one the high digit's); blocks
+// 2 p and 2 p + 1.  w: the second column's weight (256, or 0 in the odd lane).
+template <int FMT>
+__device__ __forceinline__ void product(float* acc, const Quants<FMT>& q, const Digits& f, int p, int w) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int c[4];
+    mma_s8(c, q.a[i], i ? f.b[p].z : f.b[p].x, i ? f.b[p].w : f.b[p].y);
+    const float sc = __uint_as_float(p == 0 ? (i ? f.s.y : f.s.x) : (i ? f.s.w : f.s.z));
+    acc[0] = fmaf((float)(c[0] + c[1] * w), q.d[i].x * sc, acc[0]);
+    acc[1] = fmaf((float)(c[2] + c[3] * w), q.d[i].y * sc, acc[1]);
   }
 }
 
-// f(token of the entry, first row value, second row value) for every column
-// that this lane holds after join().
-template <int MODE, typename F>
-__device__ __forceinline__ void each_col(const float (&acc)[acc_n<MODE>()], int cnt, int lane, F f) {
+// One entry's tokens against `n` groups of this warp's stream, C MMAs of
+// tokens wide.  `first`: the first group's digits of the first MMA's tokens,
+// asked for by the caller ahead of time; here the next group's are asked for
+// before the current one's products.
+template <int FMT, int DIG, int C, typename Row, typename Next>
+__device__ __forceinline__ void stream(float (&acc)[2 * C], Ring<FMT>& ring, const uint8_t* digits,
+                                       const float* scales, int groups, int g0, int n, int cnt,
+                                       int lane, const Digits& first, Row row, Next next) {
+  constexpr int T = tok_mma<DIG>(), SG = slot_groups<FMT>();
+  constexpr float Q = FMT == 8 ? 1.0f : 0.0625f;  // q4_0 quants come as 16 (n - 8)
+  const bool hi = DIG == 3 && (lane & 1);
+  const int w = hi ? 0 : 256;
+  Cols<DIG> cols[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    cols[c].set(digits, scales, groups, c ? g0 : g0 + 1, cnt - c * T, lane,
+                [&](int i) { return row(c * T + i); });
+#pragma unroll
+  for (int i = 0; i < 2 * C; ++i) acc[i] = 0.0f;
+  Digits f[2][C];  // of even and odd groups
+  f[0][0] = first;
+#pragma unroll
+  for (int c = 1; c < C; ++c) cols[c].load(f[0][c]);
+  for (int g = 0; g < n; g += SG) {
+    const uint32_t st = ring.wait();
+#pragma unroll
+    for (int j = 0; j < SG; ++j) {
+      if (j > 0 && g + j >= n) break;
+      if (g + j + 1 < n) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) cols[c].load(f[(j + 1) & 1][c]);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        Quants<FMT> q;
+        q.load(st + j * grp_bytes<FMT>(), p, lane);
+#pragma unroll
+        for (int c = 0; c < C; ++c) product<FMT>(acc + 2 * c, q, f[j & 1][c], p, w);
+      }
+    }
+    __syncwarp();  // every lane has read the slot
+    ++ring.taken;
+    ring.ask(lane, next);
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * C; ++i) {
+    acc[i] *= hi ? 65536.0f * Q : Q;
+    if (DIG == 3) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+  }
+}
+
+// f(token of the entry, first row value, second row value) for every token
+// that this lane holds.
+template <int DIG, int C, typename F>
+__device__ __forceinline__ void each_token(const float (&acc)[2 * C], int cnt, int lane, F f) {
   const int t = lane & 3;
-  if constexpr (MODE == 2) {
-    if (!(t & 1) && (t >> 1) < cnt) f(t >> 1, acc[0], acc[1]);
-  } else {
 #pragma unroll
-    for (int h = 0; h < MODE / 8; ++h)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (8 * h + 2 * t + j < cnt) f(8 * h + 2 * t + j, acc[4 * h + j], acc[4 * h + 2 + j]);
+  for (int c = 0; c < C; ++c) {
+    const int i = c * tok_mma<DIG>() + (DIG == 2 ? t : t >> 1);
+    if ((DIG == 2 || !(t & 1)) && i < cnt) f(i, acc[2 * c], acc[2 * c + 1]);
   }
+}
+
+// run(C) for the number of MMAs that cnt tokens need
+template <int DIG, typename F>
+__device__ __forceinline__ void by_width(int cnt, F run) {
+  constexpr int T = tok_mma<DIG>();
+  if (cnt <= T) run(std::integral_constant<int, 1>());
+  else run(std::integral_constant<int, 2>());
 }
 
 // ------------------------------------------------------------- gate and up
-template <int FMT>
-__global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_up(MoeArgs a) {
+// One CTA per SM, 16 warps: 4 row tiles (8 gate and 8 up rows each) x 4
+// quarters of the columns, all on one unit, so that what is left at the end
+// of the launch is a fraction of a unit per SM (4 CTAs of 4 warps with a unit
+// each: 688 units of 4096 columns in q8_0 took 40 us).  The warps' rings run
+// on into the next unit while one is finished.
+template <int DIG> struct UpPart {
+  float v[2][MOE_UPK][ent_tok<DIG>()][72];  // [buffer][quarter][token][32 gate, 32 up, padding]
+};
+template <int FMT, int DIG>
+__global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
   extern __shared__ __align__(128) uint8_t up_smem[];
-  __shared__ float hbuf[2][MOE_ENT][32];
-  constexpr int GB = grp_bytes<FMT>(), D = ring_depth<FMT>();
+  constexpr int ENT = ent_tok<DIG>(), GB = grp_bytes<FMT>(), WARPS = MOE_W * MOE_UPK;
+  __shared__ __align__(8) unsigned long long bars[WARPS][MOE_RING];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rt = warp % MOE_W, kq = warp / MOE_W;
   pdl_wait();
   pdl_trigger();
-  const Table tb = build_table(up_smem + (size_t)MOE_W * D * GB, a);
+  UpPart<DIG>& part = *reinterpret_cast<UpPart<DIG>*>(up_smem + (size_t)WARPS * ring_bytes<FMT>());
+  const Table tb = build_table<ENT>(up_smem + (size_t)WARPS * ring_bytes<FMT>() + sizeof(UpPart<DIG>), a);
   const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F);
   const int units = tb.nent * fc;
+  const int g0 = kg * kq / MOE_UPK, n = kg * (kq + 1) / MOE_UPK - g0;  // this warp's groups
   const int64_t tile = (int64_t)kg * GB;  // one 16-row tile
-  Ring<FMT> ring{saddr(up_smem) + (uint32_t)(warp * D * GB), 0, 0};
-  // the tile of unit u that this warp reads: expert, then 8-row pairs
-  auto src_of = [&](int u) {
-    const uint32_t en = tb.ent[u / fc];
-    return a.gate_up + ((int64_t)(en & 1023u) * (a.F / 8) + (u % fc) * MOE_W + warp) * tile;
+  Ring<FMT> ring;
+  ring.init(saddr(up_smem) + (uint32_t)(warp * ring_bytes<FMT>()), saddr(bars[warp]), lane);
+  // unit u: an entry and 32 rows.  An expert's entries take turns at the same
+  // rows, so that the second reads them from L2.
+  auto unit = [&](int u, int& chunk) {
+    const int e = u / fc;
+    chunk = u - e * fc;
+    const uint32_t en = tb.ent[e];
+    const int at = (en >> 26) & 63, run = tb.run(e);
+    if (run == 1) return en;
+    const int local = at * fc + chunk;
+    chunk = local / run;
+    return tb.ent[e - at + local - chunk * run];
   };
-  int pu = blockIdx.x, pg = 0;  // next group to ask for
-  const uint8_t* psrc = pu < units ? src_of(pu) : nullptr;
-  auto ask = [&]() {
-    if (pu < units) {
-      ring.fill(psrc + (int64_t)pg * GB, lane);
-      if (++pg == kg) {
-        pg = 0;
-        pu += gridDim.x;
-        if (pu < units) psrc = src_of(pu);
-      }
+  int pu = blockIdx.x;  // next unit to ask for
+  auto next = [&](const uint8_t*& src, int& left) {
+    if (pu >= units || n == 0) return false;
+    int chunk;
+    const uint32_t en = unit(pu, chunk);
+    src = a.gate_up + ((int64_t)(en & 1023u) * (a.F / 8) + chunk * MOE_W + rt) * tile + (int64_t)g0 * GB;
+    left = n;
+    pu += gridDim.x;
+    return true;
+  };
+  for (int i = 0; i < MOE_RING; ++i) ring.ask(lane, next);
+  auto row_of = [&](uint32_t en, int i) { return (int64_t)(tb.sorted[((en >> 10) & 0xFFF) + i] >> 16); };
+  // the first digits of unit u, asked for while the unit before it runs
+  Digits first;
+  auto early = [&](int u) {
+    if (u < units && n > 0) {
+      int chunk;
+      const uint32_t en = unit(u, chunk);
+      Cols<DIG> c;
+      c.set(a.xdig, a.xs, kg, g0, (en >> 22) & 15, lane, [&](int i) { return row_of(en, i); });
+      c.load(first);
     }
-    cp_commit();
   };
-  for (int i = 0; i < D; ++i) ask();
+  early(blockIdx.x);
   int buf = 0;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const uint32_t en = tb.ent[u / fc];
-    const int first = (en >> 10) & 0xFFF, cnt = en >> 22;
-    auto run = [&](auto mode) {
-      constexpr int MODE = decltype(mode)::value;
-      float acc[acc_n<MODE>()] = {};
-      Cols<FMT, MODE> cols;
-      cols.set(a.xdig, a.xs, kg, cnt, lane,
-               [&](int i) { return (int64_t)(tb.sorted[first + i] >> 16); });
-      for (int g = 0; g < kg; ++g) {
-        group_product<FMT, MODE>(acc, cols, g, ring.base + (uint32_t)(ring.out * GB), lane, [&]() {
-          cp_wait<D - 1>();
-          __syncwarp();
-        });
-        __syncwarp();  // every lane has read the slot
-        ring.out = ring.out + 1 == D ? 0 : ring.out + 1;
-        ask();
-      }
-      join<MODE>(acc);
-      each_col<MODE>(acc, cnt, lane, [&](int i, float gate, float up) {
-        const float w = tb.w[tb.sorted[first + i] & 0xFFFFu];
-        hbuf[buf][i][warp * 8 + (lane >> 2)] = gate / (1.0f + expf(-gate)) * up * w;
+    int hb;  // this unit's block of h
+    const uint32_t en = unit(u, hb);
+    const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15;
+    by_width<DIG>(cnt, [&](auto width) {
+      constexpr int C = decltype(width)::value;
+      float acc[2 * C];
+      const Digits now = first;
+      early(u + gridDim.x);
+      stream<FMT, DIG, C>(acc, ring, a.xdig, a.xs, kg, g0, n, cnt, lane, now,
+                          [&](int i) { return row_of(en, i); }, next);
+      each_token<DIG, C>(acc, cnt, lane, [&](int i, float gate, float up) {
+        float* p = part.v[buf][kq][i] + rt * 8 + (lane >> 2);
+        p[0] = gate;
+        p[32] = up;
       });
-    };
-    if (cnt <= 2) run(std::integral_constant<int, 2>());
-    else if (cnt <= 8) run(std::integral_constant<int, 8>());
-    else run(std::integral_constant<int, 16>());
+    });
     __syncthreads();
-    // the unit's 32 values of a token are block u % fc of its h
-    const int hb = u % fc;
-    for (int i = warp; i < cnt; i += MOE_W) {
-      const float v = hbuf[buf][i][lane];
+    // the unit's 32 values of a token are a block of its h: one warp per token,
+    // one value per lane
+    for (int i = warp; i < cnt; i += WARPS) {
+      float gate = 0.0f, up = 0.0f;
+#pragma unroll
+      for (int q = 0; q < MOE_UPK; ++q) {
+        gate += part.v[buf][q][i][lane];
+        up += part.v[buf][q][i][32 + lane];
+      }
+      const int64_t row = tb.sorted[at + i] & 0xFFFFu;
+      const float v = gate / (1.0f + expf(-gate)) * up * tb.w[row];
       const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7FFFFFFFu);
-      const BlockScale b = block_scale(m);
-      const uint32_t f = fixed_biased(v, b) ^ 0x808080u;
-      const int64_t row = tb.sorted[first + i] & 0xFFFFu;
-      uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * MOE_DIG + ((lane >> 2) & 3) * 32 +
+      const BlockScale b = block_scale<DIG>(m);
+      const uint32_t f = fixed_biased<DIG>(v, b) ^ 0x808080u;
+      uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * dig_bytes<DIG>() + ((lane >> 2) & 3) * 32 +
                      (hb & 3) * 8 + (lane >> 4) * 4 + (lane & 3);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
+      for (int p = 0; p < DIG; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
       if (lane == 0) a.hs[row * fg * 4 + hb] = b.scale;
     }
     buf ^= 1;  // the next unit's values go to the other buffer, so one barrier a unit is enough
   }
+  ring.finish();
 }
 
 // -------------------------------------------------------------------- down
-template <int FMT>
+// CTAs of 4 warps, each warp with 16 rows of y; a cluster's CTAs have the same
+// 64 rows and share out the columns of all the entries (entry after entry,
+// cut anywhere).
+template <int FMT, int DIG>
 __global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_down(MoeArgs a, int ydt) {
   extern __shared__ __align__(128) uint8_t dn_smem[];
-  constexpr int GB = grp_bytes<FMT>(), D = ring_depth<FMT>();
+  __shared__ __align__(8) unsigned long long bars[MOE_W][MOE_RING];
+  constexpr int GB = grp_bytes<FMT>();
   cg::cluster_group cl = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   // the choices were complete before k_moe_up passed its own wait and
   // allowed this launch; what k_moe_up writes comes after the wait below
   const size_t yb = (size_t)a.N * 16 * MOE_W * 4;
-  float* ypart = reinterpret_cast<float*>(dn_smem + (size_t)MOE_W * D * GB);
-  const Table tb = build_table(dn_smem + (size_t)MOE_W * D * GB + yb, a);
+  float* ypart = reinterpret_cast<float*>(dn_smem + (size_t)MOE_W * ring_bytes<FMT>());
+  const Table tb = build_table<ent_tok<DIG>()>(dn_smem + (size_t)MOE_W * ring_bytes<FMT>() + yb, a);
   const int fg = groups_of(a.F);
   const int64_t total = (int64_t)tb.nent * fg;
   const int q0 = (int)(total * rank / cs), q1 = (int)(total * (rank + 1) / cs);
   const int rt = blockIdx.x / cs * MOE_W + warp, nrt = a.K / 16;  // this warp's 16 rows
-  const bool live = rt < nrt;
+  const bool live = rt < nrt && q0 < q1;
   const int64_t tile = (int64_t)fg * GB;
-  Ring<FMT> ring{saddr(dn_smem) + (uint32_t)(warp * D * GB), 0, 0};
-  auto src_of = [&](int en) {
-    return a.down + ((int64_t)(tb.ent[en] & 1023u) * nrt + rt) * tile;
+  Ring<FMT> ring;
+  ring.init(saddr(dn_smem) + (uint32_t)(warp * ring_bytes<FMT>()), saddr(bars[warp]), lane);
+  int pq = live ? q0 : q1;
+  auto next = [&](const uint8_t*& src, int& left) {
+    if (pq >= q1) return false;
+    const int e = pq / fg, g = pq - e * fg;
+    src = a.down + ((int64_t)(tb.ent[e] & 1023u) * nrt + rt) * tile + (int64_t)g * GB;
+    left = min(fg - g, q1 - pq);
+    pq += left;
+    return true;
   };
-  int pq = q0, pe = q0 / fg, pg = q0 % fg;
-  const uint8_t* psrc = live && q0 < q1 ? src_of(pe) : nullptr;
-  auto ask = [&]() {
-    if (live && pq < q1) {
-      ring.fill(psrc + (int64_t)pg * GB, lane);
-      ++pq;
-      if (++pg == fg) {
-        pg = 0;
-        ++pe;
-        if (pq < q1) psrc = src_of(pe);
-      }
-    }
-    cp_commit();
-  };
-  for (int i = 0; i < D; ++i) ask();
+  for (int i = 0; i < MOE_RING; ++i) ring.ask(lane, next);
   for (int i = threadIdx.x; i < a.N * 16 * MOE_W; i += 32 * MOE_W) ypart[i] = 0.0f;
   __syncthreads();
   pdl_wait();
   pdl_trigger();
   if (live) {
+    auto row_of = [&](uint32_t en, int i) { return (int64_t)(tb.sorted[((en >> 10) & 0xFFF) + i] & 0xFFFFu); };
+    // the first digits of the entry that group q belongs to, from q on
+    Digits first;
+    auto early = [&](int q) {
+      if (q < q1) {
+        const int e = q / fg;
+        const uint32_t en = tb.ent[e];
+        Cols<DIG> c;
+        c.set(a.hdig, a.hs, fg, q - e * fg, (en >> 22) & 15, lane, [&](int i) { return row_of(en, i); });
+        c.load(first);
+      }
+    };
+    early(q0);
     for (int q = q0; q < q1;) {
-      const int e = q / fg, g0 = q % fg, g1 = min(fg, g0 + q1 - q);
+      const int e = q / fg, g0 = q - e * fg, n = min(fg - g0, q1 - q);
       const uint32_t en = tb.ent[e];
-      const int first = (en >> 10) & 0xFFF, cnt = en >> 22;
-      auto run = [&](auto mode) {
-        constexpr int MODE = decltype(mode)::value;
-        float acc[acc_n<MODE>()] = {};
-        Cols<FMT, MODE> cols;
-        cols.set(a.hdig, a.hs, fg, cnt, lane,
-                 [&](int i) { return (int64_t)(tb.sorted[first + i] & 0xFFFFu); });
-        for (int g = g0; g < g1; ++g) {
-          group_product<FMT, MODE>(acc, cols, g, ring.base + (uint32_t)(ring.out * GB), lane, [&]() {
-            cp_wait<D - 1>();
-            __syncwarp();
-          });
-          __syncwarp();
-          ring.out = ring.out + 1 == D ? 0 : ring.out + 1;
-          ask();
-        }
-        join<MODE>(acc);
+      const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15;
+      by_width<DIG>(cnt, [&](auto width) {
+        constexpr int C = decltype(width)::value;
+        float acc[2 * C];
+        const Digits now = first;
+        early(q + n);
+        stream<FMT, DIG, C>(acc, ring, a.hdig, a.hs, fg, g0, n, cnt, lane, now,
+                            [&](int i) { return row_of(en, i); }, next);
         // tokens of an entry are distinct, and the rows are this warp's own
-        each_col<MODE>(acc, cnt, lane, [&](int i, float lo, float hi) {
-          float* p = ypart + (tb.sorted[first + i] >> 16) * 16 * MOE_W + warp * 16 + (lane >> 2);
+        each_token<DIG, C>(acc, cnt, lane, [&](int i, float lo, float hi) {
+          float* p = ypart + (tb.sorted[at + i] >> 16) * 16 * MOE_W + warp * 16 + (lane >> 2);
           p[0] += lo;
           p[8] += hi;
         });
-      };
-      if (cnt <= 2) run(std::integral_constant<int, 2>());
-      else if (cnt <= 8) run(std::integral_constant<int, 8>());
-      else run(std::integral_constant<int, 16>());
+      });
       __syncwarp();  // the next entry may add to the same token from other lanes
-      q += g1 - g0;
+      q += n;
     }
   }
+  ring.finish();
   cl.sync();
   const int row0 = blockIdx.x / cs * 16 * MOE_W;
   for (int i = rank * 32 * MOE_W + threadIdx.x; i < a.N * 16 * MOE_W; i += cs * 32 * MOE_W) {
@@ -976,11 +1112,11 @@ WsMap ws_map(int64_t N, int slots, int64_t K, int64_t F) {
   m.weights = o;
   o += up(n * slots * 4);
   m.xdig = o;
-  o += up(n * kg * MOE_DIG);
+  o += up(n * kg * dig_bytes<3>());
   m.xs = o;
   o += up(n * kg * 16);
   m.hdig = o;
-  o += up(n * slots * fg * MOE_DIG);
+  o += up(n * slots * fg * dig_bytes<3>());
   m.hs = o;
   o += up(n * slots * fg * 16);
   m.bytes = o;
@@ -1012,53 +1148,73 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
   return OK;
 }
 
+// Clusters of more than 8 CTAs are opt-in per kernel (and device).
+int allow_cluster16(const void* f, const DeviceInfo& dev) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_pair(f, dev.device);
+  if (done.count(key)) return OK;
+  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return set_error(ERR_CUDA, "allowing clusters of 16: %s", cudaGetErrorString(e));
+  done.insert(key);
+  return OK;
+}
+
 template <int TN>
 size_t route_smem(int E) {
-  const int epad = (E + RT_CL - 1) / RT_CL;
+  const int epad = (E + rt_cl<TN>() - 1) / rt_cl<TN>();
   return (size_t)TN * rt_chunk<TN>() * 8 + (size_t)RT_WARPS * epad * TN * 8 + (size_t)E * 12;
 }
 
-// Routing and / or the fixed-point form of x: one launch.
-int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const DeviceInfo& dev,
-                 cudaStream_t st) {
-  const int tn = a.N == 1 ? 1 : 8;
-  r.clusters = route ? (a.N + tn - 1) / tn : 0;
+template <int TN>
+int launch_route_n(const MoeArgs& a, RouteArgs& r, bool route, bool prep, const DeviceInfo& dev,
+                   cudaStream_t st) {
+  constexpr int CL = rt_cl<TN>();
+  r.clusters = route ? (a.N + TN - 1) / TN : 0;
   // one warp per token and group, at most two CTAs per SM, in whole clusters
   int pre = 0;
   if (prep) {
     const int64_t warps = (int64_t)a.N * groups_of(a.K);
     pre = (int)std::min<int64_t>((warps + RT_WARPS - 1) / RT_WARPS, 2 * dev.sms);
-    pre = (pre + RT_CL - 1) / RT_CL * RT_CL;
+    pre = (pre + CL - 1) / CL * CL;
   }
-  const dim3 grid(RT_CL * r.clusters + pre);
-  const void* f = tn == 1 ? (const void*)k_moe_route<1> : (const void*)k_moe_route<8>;
-  if (int rc = allow_max_smem(f, dev)) return rc;
-  const size_t smem = route ? (tn == 1 ? route_smem<1>(r.E) : route_smem<8>(r.E)) : 0;
-  if (tn == 1) return launch("k_moe_route", k_moe_route<1>, grid, RT_THREADS, smem, RT_CL, st, a, r);
-  return launch("k_moe_route", k_moe_route<8>, grid, RT_THREADS, smem, RT_CL, st, a, r);
+  if (int rc = allow_max_smem((const void*)k_moe_route<TN>, dev)) return rc;
+  if (CL > 8)
+    if (int rc = allow_cluster16((const void*)k_moe_route<TN>, dev)) return rc;
+  return launch("k_moe_route", k_moe_route<TN>, dim3(CL * r.clusters + pre), RT_THREADS,
+                route ? route_smem<TN>(r.E) : 0, CL, st, a, r);
 }
 
-template <int FMT>
+// Routing and / or the fixed-point form of x: one launch.
+int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const DeviceInfo& dev,
+                 cudaStream_t st) {
+  // up to 32 tokens two to a cluster (latency counts: the clusters run side by
+  // side), above that eight (the router's weights are read an eighth as often)
+  if (a.N == 1) return launch_route_n<1>(a, r, route, prep, dev, st);
+  if (a.N <= 32) return launch_route_n<2>(a, r, route, prep, dev, st);
+  return launch_route_n<8>(a, r, route, prep, dev, st);
+}
+
+template <int FMT, int DIG>
 int launch_up(const MoeArgs& a, const DeviceInfo& dev, cudaStream_t st) {
-  if (int rc = allow_max_smem((const void*)k_moe_up<FMT>, dev)) return rc;
-  const size_t smem = (size_t)MOE_W * ring_depth<FMT>() * grp_bytes<FMT>() +
+  if (int rc = allow_max_smem((const void*)k_moe_up<FMT, DIG>, dev)) return rc;
+  const size_t smem = (size_t)MOE_W * MOE_UPK * ring_bytes<FMT>() + sizeof(UpPart<DIG>) +
                       table_bytes(a.E, a.N * a.slots, a.max_ent);
-  int occ = 0;
-  if (int rc = occupancy((const void*)k_moe_up<FMT>, dev, 32 * MOE_W, smem, &occ)) return rc;
   const int64_t units = (int64_t)a.max_ent * (a.F / 32);
-  const dim3 grid((unsigned)std::min<int64_t>(units, (int64_t)dev.sms * occ));
-  return launch("k_moe_up", k_moe_up<FMT>, grid, 32 * MOE_W, smem, 0, st, a);
+  const dim3 grid((unsigned)std::min<int64_t>(units, dev.sms));
+  return launch("k_moe_up", k_moe_up<FMT, DIG>, grid, UP_THREADS, smem, 0, st, a);
 }
 
-template <int FMT>
+template <int FMT, int DIG>
 int launch_down(const MoeArgs& a, int ydt, const DeviceInfo& dev, cudaStream_t st) {
-  if (int rc = allow_max_smem((const void*)k_moe_down<FMT>, dev)) return rc;
-  const size_t smem = (size_t)MOE_W * ring_depth<FMT>() * grp_bytes<FMT>() +
+  if (int rc = allow_max_smem((const void*)k_moe_down<FMT, DIG>, dev)) return rc;
+  const size_t smem = (size_t)MOE_W * ring_bytes<FMT>() +
                       (size_t)a.N * 16 * MOE_W * 4 + table_bytes(a.E, a.N * a.slots, a.max_ent);
   const int chunks = (a.K / 16 + MOE_W - 1) / MOE_W;
-  int cs = 1;  // CTAs that share 64 rows: as many as the device holds at once
-  while (cs < 8 && chunks * cs * 2 <= dev.sms * 4) cs *= 2;
-  return launch("k_moe_down", k_moe_down<FMT>, dim3(chunks * cs), 32 * MOE_W, smem, cs, st, a, ydt);
+  // CTAs that share 64 rows: as many as the device holds at once, four per SM
+  const int cs = std::max(1, std::min(MOE_DOWN_CL, dev.sms * 4 / chunks));
+  return launch("k_moe_down", k_moe_down<FMT, DIG>, dim3(chunks * cs), 32 * MOE_W, smem, cs, st, a, ydt);
 }
 
 }  // namespace
@@ -1146,7 +1302,7 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
     a.F = (int)m.F;
     // every entry but an expert's last is full
     const int P = a.N * slots;
-    a.max_ent = std::min(m.E, P) + P / MOE_ENT;
+    a.max_ent = std::min(m.E, P) + P / (xdt == 0 ? ent_tok<3>() : ent_tok<2>());
     a.y = static_cast<uint8_t*>(y) + n0 * ldy * xb;
     a.ldy = ldy;
     RouteArgs r = {};
@@ -1166,10 +1322,37 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
       r.weights = reinterpret_cast<float*>(w + wm.weights);
     }
     if (int rc = launch_route(a, r, route != nullptr, true, dev, st)) return rc;
-    if (int rc = m.fmt == 8 ? launch_up<8>(a, dev, st) : launch_up<4>(a, dev, st)) return rc;
-    if (int rc = m.fmt_down == 8 ? launch_down<8>(a, xdt, dev, st) : launch_down<4>(a, xdt, dev, st))
-      return rc;
+    int rc;
+    if (xdt == 0) rc = m.fmt == 8 ? launch_up<8, 3>(a, dev, st) : launch_up<4, 3>(a, dev, st);
+    else rc = m.fmt == 8 ? launch_up<8, 2>(a, dev, st) : launch_up<4, 2>(a, dev, st);
+    if (rc) return rc;
+    if (xdt == 0) rc = m.fmt_down == 8 ? launch_down<8, 3>(a, xdt, dev, st) : launch_down<4, 3>(a, xdt, dev, st);
+    else rc = m.fmt_down == 8 ? launch_down<8, 2>(a, xdt, dev, st) : launch_down<4, 2>(a, xdt, dev, st);
+    if (rc) return rc;
   }
+  return OK;
+}
+
+int set_moe_spin_limit(long long cycles) {
+  const cudaError_t e = cudaMemcpyToSymbol(g_moe_spin_limit, &cycles, sizeof(cycles));
+  if (e == cudaSuccess) return OK;
+  return set_error(ERR_CUDA, "setting the wait limit: %s", cudaGetErrorString(e));
+}
+
+int read_moe_error(int clear, cudaStream_t st, int* out) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_moe_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess)
+    return set_error(ERR_CUDA, "reading the device error word: %s", cudaGetErrorString(e));
+  if (clear && v) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_moe_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess)
+      return set_error(ERR_CUDA, "clearing the device error word: %s", cudaGetErrorString(e));
+  }
+  *out = v;
   return OK;
 }
 

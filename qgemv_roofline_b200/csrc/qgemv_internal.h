@@ -219,6 +219,8 @@ int int8_quantize(const void* x, int xdt, int64_t ldx, int64_t N, int64_t K, voi
 // early_w: the launch before this one was int8_quantize's on the same stream
 // (the weights may be read before it has finished).
 int int8_matmul(const Int8Call& c, bool early_w, cudaStream_t st);
+int set_moe_spin_limit(long long cycles);
+int read_moe_error(int clear, cudaStream_t st, int* out);
 int set_i8_spin_limit(long long cycles);
 int read_i8_error(int clear, cudaStream_t st, int* out);
 
