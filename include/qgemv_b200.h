@@ -535,7 +535,8 @@ QGEMV_API int qgemv_mg_destroy(void* handle);
 #define QGEMV_SIGMOID 1
 
 /* Expert tiles: the layout that the kernels stream, made once per weight
- * (16 rows x 128 columns in matrix-fragment order; columns padded to 128).
+ * (16 rows x 128 columns in matrix-fragment order; rows padded to 64, columns
+ * to 128).
  * Bytes of E experts' [rows, cols] matrices; gate and up together count as
  * one matrix of 2 F rows.  0 when rows % 16 or cols % 32 is not 0. */
 QGEMV_API size_t qgemv_moe_tiles_bytes(int format, int64_t n_experts, int64_t rows, int64_t cols);

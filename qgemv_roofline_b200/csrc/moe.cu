@@ -14,13 +14,19 @@
 //    order of the sum), exchanged through distributed shared memory, then the
 //    top k of each token by one warp.  Further CTAs of the same launch round x
 //    to block fixed point (below).
-//  * k_moe_up: work units of one expert x 32 h rows.  Each of a CTA's 4 warps
-//    streams 8 gate rows and the same 8 up rows as one 16-row MMA tile, so
-//    silu(gate) * up is lane-local; the unit's 32 h values of a token are one
-//    block of the down projection, rounded to fixed point right there.
-//  * k_moe_down: a CTA owns 64 rows of y (16 per warp); a cluster of CTAs
-//    splits the chosen experts' columns and adds its parts through distributed
-//    shared memory in rank order (deterministic).
+//  * k_moe_up: work units of one expert x 32 h rows.  A warp's 16-row MMA tile is
+//    8 gate rows and the same 8 up rows; the unit's 32 h values of a token are
+//    one block of the down projection and are rounded to fixed point right
+//    there.
+//  * k_moe_down: a CTA owns 64 rows of y; a cluster of CTAs splits the chosen
+//    experts' columns and adds its parts through distributed shared memory in
+//    rank order (deterministic).
+//
+// Both stream their weights the same way: one CTA per SM, a producer warp that
+// fills a ring of 9 stages with bulk copies (a stage is a slab: 4 row tiles x 2
+// or 4 groups of 128 columns, 17 or 18 KB in one contiguous piece), and 12
+// compute warps, one per row tile and one of three splits: split s takes every
+// third slab.  Every wait is bounded.
 //
 // The arithmetic is the library's exact-integer scheme.  A block of 32
 // activations is rounded to integers X = rint(x FX / max |x|) and split into
@@ -42,14 +48,14 @@
 // (|S0 + 2^8 S1| < 2^28) and converted once.
 // A block that holds a NaN or an infinity gets a NaN scale: y is NaN there.
 //
-// Weights are "expert tiles", laid out once: per expert, 16-row tiles; a
-// tile's groups of 128 columns are consecutive, each group the four blocks'
-// quants in MMA fragment order (one 16-byte shared-memory load per lane is a
-// q8_0 A fragment, or two of q4_0) and then the scales [8 rows][4 blocks][row,
-// row + 8].  q4_0 nibbles are stored with bit 3 flipped: n ^ 8 shifted into
-// the high half of a byte is 16 (n - 8) as a signed byte, one or two
-// instructions; the 1/16 is folded into the activation scale (exact).  A warp
-// reads its tile as one contiguous stream through a private ring of bulk copies.
+// Weights are "expert tiles", laid out once: per expert, chunks of 64 rows (four
+// 16-row tiles; rows past the last are zero); a chunk's groups of 128 columns
+// follow one another, each the four tiles' pieces; a tile's piece is its four
+// blocks' quants in MMA fragment order (one 16-byte shared-memory load per lane
+// is a q8_0 A fragment, or two of q4_0) and then the scales [8 rows][4 blocks]
+// [row, row + 8].  q4_0 nibbles are stored with bit 3 flipped: n ^ 8 shifted
+// into the high half of a byte is 16 (n - 8) as a signed byte, one or two
+// instructions; the 1/16 is folded into the result's factor (exact).
 #include <algorithm>
 #include <mutex>
 #include <set>
@@ -72,10 +78,13 @@ __device__ long long g_moe_spin_limit = kDefaultSpinLimit;
 namespace {
 
 constexpr int MOE_NT = kMoeTokens;  // tokens per pass
-constexpr int MOE_W = 4;            // row tiles (of 16) that a CTA's warps take side by side
-constexpr int MOE_UPK = 4;          // gate / up: warps that split a row tile's columns
-constexpr int MOE_DOWN_CL = 8;      // down: CTAs of a cluster, at most
-constexpr int UP_THREADS = 32 * MOE_W * MOE_UPK;
+constexpr int MOE_RT = 4;                  // row tiles (of 16) of a slab, one per compute warp
+constexpr int MOE_KS = 3;                  // compute warps per row tile
+constexpr int MOE_CW = MOE_RT * MOE_KS;    // compute warps; then the producer
+constexpr int MOE_EW = 3;                  // gate / up: warps that finish units
+constexpr int UP_THREADS = 32 * (MOE_CW + 1 + MOE_EW);
+constexpr int DN_THREADS = 32 * (MOE_CW + 1);
+constexpr int MOE_DOWN_CL = 8;             // down: CTAs of a cluster, at most
 constexpr int MOE_GCOLS = 128;      // columns of a group (4 blocks)
 // digit bytes of a group: [digits][4 lanes][32]
 template <int DIG> __host__ __device__ constexpr int dig_bytes() { return DIG * 128; }
@@ -88,12 +97,14 @@ template <int DIG> __host__ __device__ constexpr int ent_tok() { return 2 * tok_
 // bytes of a group (16 rows x 128 columns): quants, then 64 fp16 scales
 template <int FMT> __host__ __device__ constexpr int grp_q() { return FMT == 8 ? 2048 : 1024; }
 template <int FMT> __host__ __device__ constexpr int grp_bytes() { return grp_q<FMT>() + 128; }
-// Ring of a warp: two slots of 2 (q8_0) or 4 (q4_0) groups, 9 KB either way,
-// 144 KB on an SM of 16 warps
-constexpr int MOE_RING = 2;
-template <int FMT> __host__ __device__ constexpr int slot_groups() { return FMT == 8 ? 2 : 4; }
-template <int FMT> __host__ __device__ constexpr int slot_bytes() { return slot_groups<FMT>() * grp_bytes<FMT>(); }
-template <int FMT> __host__ __device__ constexpr int ring_bytes() { return MOE_RING * slot_bytes<FMT>(); }
+// A slab: 4 row tiles x SG groups; 9 stages are 153 or 162 KB.  The number of
+// stages is a multiple of the splits, so that a stage always belongs to the
+// same split: a warp knows a barrier's phase from its own slabs only.
+constexpr int MOE_S = 9;
+static_assert(MOE_S % MOE_KS == 0, "a stage serves one split");
+template <int FMT> __host__ __device__ constexpr int slab_groups() { return FMT == 8 ? 2 : 4; }
+template <int FMT> __host__ __device__ constexpr int slab_bytes() { return MOE_RT * slab_groups<FMT>() * grp_bytes<FMT>(); }
+template <int FMT> __host__ __device__ constexpr int ring_bytes() { return MOE_S * slab_bytes<FMT>(); }
 
 __host__ __device__ constexpr int groups_of(int64_t cols) {
   return (int)((cols + MOE_GCOLS - 1) / MOE_GCOLS);
@@ -591,19 +602,25 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
 __device__ __forceinline__ long long moe_spin_limit() {
   return *(volatile long long*)&g_moe_spin_limit;
 }
-// Bounded wait for a copy.  One that runs out is reported and the warp goes on
-// (its results are lost); `late` makes it wait again for what is in flight
-// before it ends.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity) {
+// Bounded wait; gives up at once when another thread raised the abort flag.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   const long long t0 = clock64(), lim = moe_spin_limit();
   while (!mbar_try(bar, parity)) {
+    if (*abort_flag) return false;
     if (clock64() - t0 > lim) {
       atomicExch(&g_moe_error, (int)ERR_TIMEOUT);
-      return true;
+      __threadfence();
+      *abort_flag = 1;
+      return false;
     }
   }
-  return false;
+  return true;
 }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try(bar, parity) || wait_slow(bar, parity, abort_flag);
+}
+// Wait for a copy in flight before the CTA ends: ignores the abort flag,
+// bounded by at least the default limit.
 __device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
   const long long t0 = clock64(), lim = max(moe_spin_limit(), kDefaultSpinLimit);
   while (!mbar_try(bar, parity) && clock64() - t0 < lim) {
@@ -634,56 +651,56 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint
         "r"(0));
 }
 
-// One warp's ring over a stream of groups, filled a whole ring ahead by bulk
-// copies.  The stream is a list of contiguous segments: `next(src, n)` gives
-// the next segment's first byte and its number of groups, false at the end.  A
-// slot never holds groups of two segments.
+// The stages' barriers of a CTA, and the parts of a unit (gate and up).
+struct Pipe {
+  unsigned long long full[MOE_S], empty[MOE_S], pfull[2], pempty[2];
+  int abort_flag;
+  __device__ __forceinline__ void init() {
+    for (int s = 0; s < MOE_S; ++s) {
+      mbar_init(saddr(&full[s]), 1);
+      mbar_init(saddr(&empty[s]), MOE_RT);  // the row tiles' warps of the slab's split
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(saddr(&pfull[b]), MOE_CW);
+      mbar_init(saddr(&pempty[b]), MOE_EW);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+};
+
+// A compute warp's place in the ring: stages kq, kq + 3, ... in turn.
+struct Turn {
+  int s;
+  uint32_t phase = 0u;
+  __device__ __forceinline__ void next() {
+    s += MOE_KS;
+    if (s >= MOE_S) {
+      s -= MOE_S;
+      phase ^= 1u;
+    }
+  }
+};
+
+// The producer thread's side: slab after slab into stages 0, 1, ...
 template <int FMT>
-struct Ring {
-  uint32_t base, bar;   // shared addresses of the slots and their barriers
-  int asked, taken;     // slots so far
-  const uint8_t* src;   // next group
-  int left;             // groups left in the segment
-  bool late;
-  static constexpr int SG = slot_groups<FMT>(), GB = grp_bytes<FMT>(), SB = slot_bytes<FMT>();
-  __device__ __forceinline__ void init(uint32_t slots, uint32_t bars, int lane) {
-    base = slots;
-    bar = bars;
-    asked = taken = 0;
-    src = nullptr;
-    left = 0;
-    late = false;
-    if (lane == 0) {
-      for (int i = 0; i < MOE_RING; ++i) mbar_init(bar + 8 * i, 1);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
+struct Feed {
+  Pipe& p;
+  uint32_t ring;
+  int i = 0;  // slabs so far
+  // m groups at src; false once the launch gave up
+  __device__ __forceinline__ bool put(const uint8_t* src, int m) {
+    const int s = i % MOE_S;
+    if (i >= MOE_S && !mbar_wait(saddr(&p.empty[s]), (uint32_t)(i / MOE_S - 1) & 1u, &p.abort_flag)) return false;
+    const uint32_t bytes = (uint32_t)(m * MOE_RT * grp_bytes<FMT>());
+    mbar_expect_tx(saddr(&p.full[s]), bytes);
+    bulk_g2s(ring + s * slab_bytes<FMT>(), src, bytes, saddr(&p.full[s]));
+    ++i;
+    return true;
   }
-  template <typename Next>
-  __device__ __forceinline__ void ask(int lane, Next next) {
-    if (left == 0 && !next(src, left)) left = -1;
-    if (left > 0) {
-      const int m = min(SG, left), s = asked % MOE_RING;
-      if (lane == 0) {
-        mbar_expect_tx(bar + 8 * s, (uint32_t)(m * GB));
-        bulk_g2s(base + s * SB, src, (uint32_t)(m * GB), bar + 8 * s);
-      }
-      src += m * GB;
-      left -= m;
-      ++asked;
-    }
-  }
-  // the address of the next slot in turn, once its copy has landed
-  __device__ __forceinline__ uint32_t wait() {
-    const int s = taken % MOE_RING;
-    const uint32_t parity = (uint32_t)(taken / MOE_RING) & 1u;
-    if (!mbar_try(bar + 8 * s, parity)) late |= wait_slow(bar + 8 * s, parity);
-    return base + s * SB;
-  }
+  // no copy outlives the CTA, whatever the other warps gave up on
   __device__ __forceinline__ void finish() {
-    if (__any_sync(0xffffffffu, late))
-      for (int i = max(0, asked - MOE_RING); i < asked; ++i)
-        drain(bar + 8 * (i % MOE_RING), (uint32_t)(i / MOE_RING) & 1u);
+    for (int k = max(0, i - MOE_S); k < i; ++k) drain(saddr(&p.full[k % MOE_S]), (uint32_t)(k / MOE_S) & 1u);
   }
 };
 
@@ -735,24 +752,22 @@ struct Cols {
   const uint8_t* dig;
   const float* s;
   // row(i): the activation row of the i-th of `cnt` tokens; the columns of
-  // absent tokens repeat the last one's.  g0: the first group.
+  // absent tokens repeat the last one's
   template <typename Row>
-  __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups, int g0,
-                                      int cnt, int lane, Row row) {
+  __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups, int cnt,
+                                      int lane, Row row) {
     const int n = lane >> 2, t = lane & 3;
     // three digits: column 3 (and 7) is idle and reads digit 2 again; its
     // accumulator is dropped
     const int tok = DIG == 2 ? n >> 1 : n >> 2, d = DIG == 2 ? n & 1 : min(n & 3, 2);
-    dig = digits + (row(min(tok, cnt - 1)) * groups + g0) * dig_bytes<DIG>() + d * 128 + t * 32;
-    s = scales + (row(min(DIG == 2 ? t : t >> 1, cnt - 1)) * groups + g0) * 4;
+    dig = digits + row(min(tok, cnt - 1)) * groups * dig_bytes<DIG>() + d * 128 + t * 32;
+    s = scales + row(min(DIG == 2 ? t : t >> 1, cnt - 1)) * groups * 4;
   }
-  // the digits of the next group in turn
-  __device__ __forceinline__ void load(Digits& f) {
-    f.b[0] = ldg128(dig);
-    f.b[1] = ldg128(dig + 16);
-    f.s = ldg128(s);
-    dig += dig_bytes<DIG>();
-    s += 4;
+  __device__ __forceinline__ void load(Digits& f, int grp) const {
+    const uint8_t* p = dig + grp * dig_bytes<DIG>();
+    f.b[0] = ldg128(p);
+    f.b[1] = ldg128(p + 16);
+    f.s = ldg128(s + grp * 4);
   }
 };
 
@@ -771,265 +786,305 @@ __device__ __forceinline__ void product(float* acc, const Quants<FMT>& q, const 
   }
 }
 
-// One entry's tokens against `n` groups of this warp's stream, C MMAs of
-// tokens wide.  `first`: the first group's digits of the first MMA's tokens,
-// asked for by the caller ahead of time; here the next group's are asked for
-// before the current one's products.
-template <int FMT, int DIG, int C, typename Row, typename Next>
-__device__ __forceinline__ void stream(float (&acc)[2 * C], Ring<FMT>& ring, const uint8_t* digits,
-                                       const float* scales, int groups, int g0, int n, int cnt,
-                                       int lane, const Digits& first, Row row, Next next) {
-  constexpr int T = tok_mma<DIG>(), SG = slot_groups<FMT>();
-  constexpr float Q = FMT == 8 ? 1.0f : 0.0625f;  // q4_0 quants come as 16 (n - 8)
-  const bool hi = DIG == 3 && (lane & 1);
-  const int w = hi ? 0 : 256;
-  Cols<DIG> cols[C];
+// What a compute warp holds: its entry's tokens (one or two MMAs of them),
+// their digits of two groups in turn, and its 16 rows' sums.
+template <int FMT, int DIG>
+struct Work {
+  static constexpr int T = tok_mma<DIG>(), SG = slab_groups<FMT>();
+  Cols<DIG> c0, c1;
+  Digits f[2][2];  // [even, odd group][MMA]
+  float acc[4];
+  bool two;
+  // the entry's tokens; row(i) as in Cols
+  template <typename Row>
+  __device__ __forceinline__ void entry(const uint8_t* digits, const float* scales, int groups, int cnt,
+                                        int lane, Row row) {
+    two = cnt > T;
+    c0.set(digits, scales, groups, cnt, lane, row);
+    if (two) c1.set(digits, scales, groups, cnt - T, lane, [&](int i) { return row(T + i); });
+  }
+  __device__ __forceinline__ void load(int buf, int grp) {
+    c0.load(f[buf][0], grp);
+    if (two) c1.load(f[buf][1], grp);
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    cols[c].set(digits, scales, groups, c ? g0 : g0 + 1, cnt - c * T, lane,
-                [&](int i) { return row(c * T + i); });
-#pragma unroll
-  for (int i = 0; i < 2 * C; ++i) acc[i] = 0.0f;
-  Digits f[2][C];  // of even and odd groups
-  f[0][0] = first;
-#pragma unroll
-  for (int c = 1; c < C; ++c) cols[c].load(f[0][c]);
-  for (int g = 0; g < n; g += SG) {
-    const uint32_t st = ring.wait();
+    for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
+  }
+  // m groups from grp on; the first one's digits are in f[0]
+  __device__ __forceinline__ void slab(uint32_t st, int rt, int grp, int m, int lane) {
+    const int w = DIG == 3 && (lane & 1) ? 0 : 256;
+    st += rt * grp_bytes<FMT>();
 #pragma unroll
     for (int j = 0; j < SG; ++j) {
-      if (j > 0 && g + j >= n) break;
-      if (g + j + 1 < n) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) cols[c].load(f[(j + 1) & 1][c]);
-      }
+      if (j > 0 && j >= m) break;
+      if (j + 1 < m) load((j + 1) & 1, grp + j + 1);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         Quants<FMT> q;
-        q.load(st + j * grp_bytes<FMT>(), p, lane);
-#pragma unroll
-        for (int c = 0; c < C; ++c) product<FMT>(acc + 2 * c, q, f[j & 1][c], p, w);
+        q.load(st + j * MOE_RT * grp_bytes<FMT>(), p, lane);
+        product<FMT>(acc, q, f[j & 1][0], p, w);
+        if (two) product<FMT>(acc + 2, q, f[j & 1][1], p, w);
       }
     }
-    __syncwarp();  // every lane has read the slot
-    ++ring.taken;
-    ring.ask(lane, next);
   }
+  // put(token of the entry, row g's sum, row g + 8's sum) for every token that
+  // this lane holds
+  template <typename Put>
+  __device__ __forceinline__ void each(int cnt, int lane, Put put) {
+    constexpr float Q = FMT == 8 ? 1.0f : 0.0625f;  // q4_0 quants come as 16 (n - 8)
+    const int t = lane & 3;
 #pragma unroll
-  for (int i = 0; i < 2 * C; ++i) {
-    acc[i] *= hi ? 65536.0f * Q : Q;
-    if (DIG == 3) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
-  }
-}
-
-// f(token of the entry, first row value, second row value) for every token
-// that this lane holds.
-template <int DIG, int C, typename F>
-__device__ __forceinline__ void each_token(const float (&acc)[2 * C], int cnt, int lane, F f) {
-  const int t = lane & 3;
+    for (int i = 0; i < 4; ++i) {
+      acc[i] *= DIG == 3 && (t & 1) ? 65536.0f * Q : Q;
+      if (DIG == 3) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);  // the high digit's lane
+    }
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int i = c * tok_mma<DIG>() + (DIG == 2 ? t : t >> 1);
-    if ((DIG == 2 || !(t & 1)) && i < cnt) f(i, acc[2 * c], acc[2 * c + 1]);
+    for (int c = 0; c < 2; ++c) {
+      const int i = c * T + (DIG == 2 ? t : t >> 1);
+      if ((DIG == 2 || !(t & 1)) && i < cnt) put(i, acc[2 * c], acc[2 * c + 1]);
+    }
   }
-}
-
-// run(C) for the number of MMAs that cnt tokens need
-template <int DIG, typename F>
-__device__ __forceinline__ void by_width(int cnt, F run) {
-  constexpr int T = tok_mma<DIG>();
-  if (cnt <= T) run(std::integral_constant<int, 1>());
-  else run(std::integral_constant<int, 2>());
-}
+};
 
 // ------------------------------------------------------------- gate and up
-// One CTA per SM, 16 warps: 4 row tiles (8 gate and 8 up rows each) x 4
-// quarters of the columns, all on one unit, so that what is left at the end
-// of the launch is a fraction of a unit per SM (4 CTAs of 4 warps with a unit
-// each: 688 units of 4096 columns in q8_0 took 40 us).  The warps' rings run
-// on into the next unit while one is finished.
+// The compute warps leave a unit's sums (per split) in one of two buffers and
+// go on; three further warps add the splits, form h and round it.
 template <int DIG> struct UpPart {
-  float v[2][MOE_UPK][ent_tok<DIG>()][72];  // [buffer][quarter][token][32 gate, 32 up, padding]
+  float v[2][MOE_KS][ent_tok<DIG>()][72];  // [buffer][split][token][32 gate, 32 up, padding]
 };
 template <int FMT, int DIG>
 __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
   extern __shared__ __align__(128) uint8_t up_smem[];
-  constexpr int ENT = ent_tok<DIG>(), GB = grp_bytes<FMT>(), WARPS = MOE_W * MOE_UPK;
-  __shared__ __align__(8) unsigned long long bars[WARPS][MOE_RING];
+  __shared__ __align__(8) Pipe pipe;
+  constexpr int SG = slab_groups<FMT>(), GB = grp_bytes<FMT>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rt = warp % MOE_W, kq = warp / MOE_W;
+  if (threadIdx.x == 0) pipe.init();
   pdl_wait();
   pdl_trigger();
-  UpPart<DIG>& part = *reinterpret_cast<UpPart<DIG>*>(up_smem + (size_t)WARPS * ring_bytes<FMT>());
-  const Table tb = build_table<ENT>(up_smem + (size_t)WARPS * ring_bytes<FMT>() + sizeof(UpPart<DIG>), a);
-  const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F);
-  const int units = tb.nent * fc;
-  const int g0 = kg * kq / MOE_UPK, n = kg * (kq + 1) / MOE_UPK - g0;  // this warp's groups
-  const int64_t tile = (int64_t)kg * GB;  // one 16-row tile
-  Ring<FMT> ring;
-  ring.init(saddr(up_smem) + (uint32_t)(warp * ring_bytes<FMT>()), saddr(bars[warp]), lane);
-  // unit u: an entry and 32 rows.  An expert's entries take turns at the same
-  // rows, so that the second reads them from L2.
-  auto unit = [&](int u, int& chunk) {
-    const int e = u / fc;
-    chunk = u - e * fc;
-    const uint32_t en = tb.ent[e];
-    const int at = (en >> 26) & 63, run = tb.run(e);
-    if (run == 1) return en;
-    const int local = at * fc + chunk;
-    chunk = local / run;
-    return tb.ent[e - at + local - chunk * run];
+  UpPart<DIG>& part = *reinterpret_cast<UpPart<DIG>*>(up_smem + ring_bytes<FMT>());
+  const Table tb = build_table<ent_tok<DIG>()>(up_smem + ring_bytes<FMT>() + sizeof(UpPart<DIG>), a);
+  const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F), ns = (kg + SG - 1) / SG;
+  const int units = tb.nent * fc, G = gridDim.x;
+  // unit u: entry u / fc, chunk u % fc, stepped without divisions
+  struct Pos {
+    int u, e, c;
   };
-  int pu = blockIdx.x;  // next unit to ask for
-  auto next = [&](const uint8_t*& src, int& left) {
-    if (pu >= units || n == 0) return false;
-    int chunk;
-    const uint32_t en = unit(pu, chunk);
-    src = a.gate_up + ((int64_t)(en & 1023u) * (a.F / 8) + chunk * MOE_W + rt) * tile + (int64_t)g0 * GB;
-    left = n;
-    pu += gridDim.x;
-    return true;
-  };
-  for (int i = 0; i < MOE_RING; ++i) ring.ask(lane, next);
-  auto row_of = [&](uint32_t en, int i) { return (int64_t)(tb.sorted[((en >> 10) & 0xFFF) + i] >> 16); };
-  // the first digits of unit u, asked for while the unit before it runs
-  Digits first;
-  auto early = [&](int u) {
-    if (u < units && n > 0) {
-      int chunk;
-      const uint32_t en = unit(u, chunk);
-      Cols<DIG> c;
-      c.set(a.xdig, a.xs, kg, g0, (en >> 22) & 15, lane, [&](int i) { return row_of(en, i); });
-      c.load(first);
+  const int de = G / fc, dc = G - de * fc;
+  Pos pos{(int)blockIdx.x, (int)blockIdx.x / fc, (int)blockIdx.x % fc};
+  auto step = [&]() {
+    pos.u += G;
+    pos.e += de;
+    pos.c += dc;
+    if (pos.c >= fc) {
+      pos.c -= fc;
+      ++pos.e;
     }
   };
-  early(blockIdx.x);
-  int buf = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    int hb;  // this unit's block of h
-    const uint32_t en = unit(u, hb);
-    const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15;
-    by_width<DIG>(cnt, [&](auto width) {
-      constexpr int C = decltype(width)::value;
-      float acc[2 * C];
-      const Digits now = first;
-      early(u + gridDim.x);
-      stream<FMT, DIG, C>(acc, ring, a.xdig, a.xs, kg, g0, n, cnt, lane, now,
-                          [&](int i) { return row_of(en, i); }, next);
-      each_token<DIG, C>(acc, cnt, lane, [&](int i, float gate, float up) {
-        float* p = part.v[buf][kq][i] + rt * 8 + (lane >> 2);
+  // its entry and its 32 rows.  An expert's entries take turns at the same
+  // rows, so that the second reads them from L2.
+  auto unit = [&](int& chunk) {
+    const uint32_t en = tb.ent[pos.e];
+    chunk = pos.c;
+    const int at = (int)(en >> 26), run = tb.run(pos.e);
+    if (run == 1) return en;
+    const int local = at * fc + pos.c;
+    chunk = local / run;
+    return tb.ent[pos.e - at + local - chunk * run];
+  };
+  if (warp == MOE_CW) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      Feed<FMT> feed{pipe, saddr(up_smem)};
+      bool ok = true;
+      for (; pos.u < units && ok; step()) {
+        int chunk;
+        const uint32_t en = unit(chunk);
+        const uint8_t* src = a.gate_up + ((int64_t)(en & 1023u) * fc + chunk) * kg * (MOE_RT * GB);
+        for (int g = 0; g < kg && ok; g += SG) ok = feed.put(src + (int64_t)g * MOE_RT * GB, min(SG, kg - g));
+      }
+      feed.finish();
+    }
+  } else if (warp < MOE_CW) {
+    // ------------------------------------------------------------- compute
+    const int rt = warp % MOE_RT, kq = warp / MOE_RT;
+    Work<FMT, DIG> w;
+    w.clear();
+    // unit number here, slab, the unit's first slab of this split (slab i of the
+    // CTA is split i % 3's, counted on through the units)
+    int j = 0, l = kq, l0 = kq, chunk;
+    const int shift = ns % MOE_KS;
+    Turn turn{kq};
+    uint32_t en = 0;
+    auto take = [&]() {
+      en = unit(chunk);
+      const int at = (en >> 10) & 0xFFF;
+      w.entry(a.xdig, a.xs, kg, (en >> 22) & 15, lane,
+              [&](int i) { return (int64_t)(tb.sorted[at + i] >> 16); });
+      if (l < ns) w.load(0, l * SG);
+    };
+    bool more = pos.u < units;
+    if (more) take();
+    while (more) {
+      while (l < ns) {
+        if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
+        w.slab(saddr(up_smem) + turn.s * slab_bytes<FMT>(), rt, l * SG, min(SG, kg - l * SG), lane);
+        __syncwarp();  // every lane has read the stage
+        if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
+        turn.next();
+        l += MOE_KS;
+        if (l < ns) w.load(0, l * SG);
+      }
+      if (l < ns) break;  // gave up
+      // this unit's sums; the next unit's first digits are on their way meanwhile
+      const int cnt = (en >> 22) & 15, b = j & 1;
+      l0 = l0 >= shift ? l0 - shift : l0 - shift + MOE_KS;
+      l = l0;
+      if (j >= 2 && !mbar_wait(saddr(&pipe.pempty[b]), (uint32_t)(j / 2 - 1) & 1u, &pipe.abort_flag)) break;
+      w.each(cnt, lane, [&](int i, float gate, float up) {
+        float* p = part.v[b][kq][i] + rt * 8 + (lane >> 2);
         p[0] = gate;
         p[32] = up;
       });
-    });
-    __syncthreads();
-    // the unit's 32 values of a token are a block of its h: one warp per token,
-    // one value per lane
-    for (int i = warp; i < cnt; i += WARPS) {
-      float gate = 0.0f, up = 0.0f;
-#pragma unroll
-      for (int q = 0; q < MOE_UPK; ++q) {
-        gate += part.v[buf][q][i][lane];
-        up += part.v[buf][q][i][32 + lane];
-      }
-      const int64_t row = tb.sorted[at + i] & 0xFFFFu;
-      const float v = gate / (1.0f + expf(-gate)) * up * tb.w[row];
-      const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7FFFFFFFu);
-      const BlockScale b = block_scale<DIG>(m);
-      const uint32_t f = fixed_biased<DIG>(v, b) ^ 0x808080u;
-      uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * dig_bytes<DIG>() + ((lane >> 2) & 3) * 32 +
-                     (hb & 3) * 8 + (lane >> 4) * 4 + (lane & 3);
-#pragma unroll
-      for (int p = 0; p < DIG; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
-      if (lane == 0) a.hs[row * fg * 4 + hb] = b.scale;
+      w.clear();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(saddr(&pipe.pfull[b]));
+      ++j;
+      step();
+      more = pos.u < units;
+      if (more) take();
     }
-    buf ^= 1;  // the next unit's values go to the other buffer, so one barrier a unit is enough
+  } else {
+    // -------------------------------------------------------------- finish
+    for (int j = 0; pos.u < units; ++j, step()) {
+      int hb;  // the unit's block of h
+      const uint32_t en = unit(hb);
+      const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15, b = j & 1;
+      if (!mbar_wait(saddr(&pipe.pfull[b]), (uint32_t)(j / 2) & 1u, &pipe.abort_flag)) break;
+      for (int i = warp - MOE_CW - 1; i < cnt; i += MOE_EW) {
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll
+        for (int q = 0; q < MOE_KS; ++q) {
+          gate += part.v[b][q][i][lane];
+          up += part.v[b][q][i][32 + lane];
+        }
+        const int64_t row = tb.sorted[at + i] & 0xFFFFu;
+        const float v = gate / (1.0f + expf(-gate)) * up * tb.w[row];
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7FFFFFFFu);
+        const BlockScale bs = block_scale<DIG>(m);
+        const uint32_t f = fixed_biased<DIG>(v, bs) ^ 0x808080u;
+        uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * dig_bytes<DIG>() + ((lane >> 2) & 3) * 32 +
+                       (hb & 3) * 8 + (lane >> 4) * 4 + (lane & 3);
+#pragma unroll
+        for (int p = 0; p < DIG; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
+        if (lane == 0) a.hs[row * fg * 4 + hb] = bs.scale;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(saddr(&pipe.pempty[b]));
+    }
   }
-  ring.finish();
 }
 
 // -------------------------------------------------------------------- down
-// CTAs of 4 warps, each warp with 16 rows of y; a cluster's CTAs have the same
-// 64 rows and share out the columns of all the entries (entry after entry,
-// cut anywhere).
+// A cluster's CTAs have the same 64 rows of y and share out the entries' slabs,
+// entry after entry, cut anywhere; the three splits of a CTA add into a copy of
+// the 64 rows each.
 template <int FMT, int DIG>
-__global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_down(MoeArgs a, int ydt) {
+__global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) {
   extern __shared__ __align__(128) uint8_t dn_smem[];
-  __shared__ __align__(8) unsigned long long bars[MOE_W][MOE_RING];
-  constexpr int GB = grp_bytes<FMT>();
+  __shared__ __align__(8) Pipe pipe;
+  constexpr int SG = slab_groups<FMT>(), GB = grp_bytes<FMT>(), R = 16 * MOE_RT;
   cg::cluster_group cl = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank(), chunk = blockIdx.x / cs;
+  if (threadIdx.x == 0) pipe.init();
+  float* ypart = reinterpret_cast<float*>(dn_smem + ring_bytes<FMT>());  // [split][token][64]
+  const int yn = a.N * R;
+  for (int i = threadIdx.x; i < MOE_KS * yn; i += DN_THREADS) ypart[i] = 0.0f;
   // the choices were complete before k_moe_up passed its own wait and
   // allowed this launch; what k_moe_up writes comes after the wait below
-  const size_t yb = (size_t)a.N * 16 * MOE_W * 4;
-  float* ypart = reinterpret_cast<float*>(dn_smem + (size_t)MOE_W * ring_bytes<FMT>());
-  const Table tb = build_table<ent_tok<DIG>()>(dn_smem + (size_t)MOE_W * ring_bytes<FMT>() + yb, a);
-  const int fg = groups_of(a.F);
-  const int64_t total = (int64_t)tb.nent * fg;
+  const Table tb = build_table<ent_tok<DIG>()>(dn_smem + ring_bytes<FMT>() + (size_t)MOE_KS * yn * 4, a);
+  const int fg = groups_of(a.F), fs = (fg + SG - 1) / SG, chunks = (a.K + R - 1) / R;
+  const int64_t total = (int64_t)tb.nent * fs;
   const int q0 = (int)(total * rank / cs), q1 = (int)(total * (rank + 1) / cs);
-  const int rt = blockIdx.x / cs * MOE_W + warp, nrt = a.K / 16;  // this warp's 16 rows
-  const bool live = rt < nrt && q0 < q1;
-  const int64_t tile = (int64_t)fg * GB;
-  Ring<FMT> ring;
-  ring.init(saddr(dn_smem) + (uint32_t)(warp * ring_bytes<FMT>()), saddr(bars[warp]), lane);
-  int pq = live ? q0 : q1;
-  auto next = [&](const uint8_t*& src, int& left) {
-    if (pq >= q1) return false;
-    const int e = pq / fg, g = pq - e * fg;
-    src = a.down + ((int64_t)(tb.ent[e] & 1023u) * nrt + rt) * tile + (int64_t)g * GB;
-    left = min(fg - g, q1 - pq);
-    pq += left;
-    return true;
-  };
-  for (int i = 0; i < MOE_RING; ++i) ring.ask(lane, next);
-  for (int i = threadIdx.x; i < a.N * 16 * MOE_W; i += 32 * MOE_W) ypart[i] = 0.0f;
-  __syncthreads();
-  pdl_wait();
-  pdl_trigger();
-  if (live) {
-    auto row_of = [&](uint32_t en, int i) { return (int64_t)(tb.sorted[((en >> 10) & 0xFFF) + i] & 0xFFFFu); };
-    // the first digits of the entry that group q belongs to, from q on
-    Digits first;
-    auto early = [&](int q) {
-      if (q < q1) {
-        const int e = q / fg;
-        const uint32_t en = tb.ent[e];
-        Cols<DIG> c;
-        c.set(a.hdig, a.hs, fg, q - e * fg, (en >> 22) & 15, lane, [&](int i) { return row_of(en, i); });
-        c.load(first);
+  if (warp == MOE_CW) {
+    if (lane == 0) {
+      Feed<FMT> feed{pipe, saddr(dn_smem)};
+      int e = q0 / fs, l = q0 - e * fs;
+      for (int q = q0; q < q1; ++q) {
+        const uint8_t* src = a.down + (((int64_t)(tb.ent[e] & 1023u) * chunks + chunk) * fg + l * SG) * (MOE_RT * GB);
+        if (!feed.put(src, min(SG, fg - l * SG))) break;
+        if (++l == fs) {
+          l = 0;
+          ++e;
+        }
       }
+      feed.finish();
+    }
+    __syncwarp();
+    pdl_wait();
+  } else {
+    pdl_wait();
+    pdl_trigger();
+    const int rt = warp % MOE_RT, kq = warp / MOE_RT;
+    float* yp = ypart + kq * yn + rt * 16 + (lane >> 2);
+    Work<FMT, DIG> w;
+    w.clear();
+    int q = q0 + kq, e = q / fs, l = q - e * fs;
+    Turn turn{kq};
+    uint32_t en = 0;
+    auto take = [&]() {
+      en = tb.ent[e];
+      const int at = (en >> 10) & 0xFFF;
+      w.entry(a.hdig, a.hs, fg, (en >> 22) & 15, lane,
+              [&](int i) { return (int64_t)(tb.sorted[at + i] & 0xFFFFu); });
     };
-    early(q0);
-    for (int q = q0; q < q1;) {
-      const int e = q / fg, g0 = q - e * fg, n = min(fg - g0, q1 - q);
-      const uint32_t en = tb.ent[e];
+    if (q < q1) {
+      take();
+      w.load(0, l * SG);
+    }
+    while (q < q1) {
+      if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
+      w.slab(saddr(dn_smem) + turn.s * slab_bytes<FMT>(), rt, l * SG, min(SG, fg - l * SG), lane);
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
+      turn.next();
+      q += MOE_KS;
+      l += MOE_KS;
+      if (l < fs && q < q1) {
+        w.load(0, l * SG);
+        continue;
+      }
+      // the entry's last slab of this warp: its sums, the next entry's first
+      // digits on their way meanwhile
       const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15;
-      by_width<DIG>(cnt, [&](auto width) {
-        constexpr int C = decltype(width)::value;
-        float acc[2 * C];
-        const Digits now = first;
-        early(q + n);
-        stream<FMT, DIG, C>(acc, ring, a.hdig, a.hs, fg, g0, n, cnt, lane, now,
-                            [&](int i) { return row_of(en, i); }, next);
-        // tokens of an entry are distinct, and the rows are this warp's own
-        each_token<DIG, C>(acc, cnt, lane, [&](int i, float lo, float hi) {
-          float* p = ypart + (tb.sorted[at + i] >> 16) * 16 * MOE_W + warp * 16 + (lane >> 2);
-          p[0] += lo;
-          p[8] += hi;
-        });
+      if (q < q1) {
+        while (l >= fs) {
+          l -= fs;
+          ++e;
+        }
+        take();
+        w.load(0, l * SG);
+      }
+      // tokens of an entry are distinct, and the rows are this warp's own
+      w.each(cnt, lane, [&](int k, float lo, float hi) {
+        float* p = yp + (tb.sorted[at + k] >> 16) * R;
+        p[0] += lo;
+        p[8] += hi;
       });
+      w.clear();
       __syncwarp();  // the next entry may add to the same token from other lanes
-      q += n;
     }
   }
-  ring.finish();
   cl.sync();
-  const int row0 = blockIdx.x / cs * 16 * MOE_W;
-  for (int i = rank * 32 * MOE_W + threadIdx.x; i < a.N * 16 * MOE_W; i += cs * 32 * MOE_W) {
+  for (int i = rank * DN_THREADS + threadIdx.x; i < yn; i += cs * DN_THREADS) {
     float v = 0.0f;
-    for (int c = 0; c < cs; ++c) v += cl.map_shared_rank(ypart, c)[i];
-    const int n = i / (16 * MOE_W), row = row0 + i % (16 * MOE_W);
+    for (int c = 0; c < cs; ++c) {
+      const float* p = cl.map_shared_rank(ypart, c) + i;
+#pragma unroll
+      for (int s = 0; s < MOE_KS; ++s) v += p[s * yn];
+    }
+    const int n = i / R, row = chunk * R + i % R;
     if (row < a.K) {
       const int64_t o = (int64_t)n * a.ldy + row;
       if (ydt == 0) static_cast<float*>(a.y)[o] = v;
@@ -1041,8 +1096,8 @@ __global__ void __launch_bounds__(32 * MOE_W, 4) k_moe_down(MoeArgs a, int ydt) 
 }
 
 // ------------------------------------------------------------ expert tiles
-// One warp per group: 16 rows (of one matrix, or 8 of each of two) x 128
-// columns of one expert; blocks past the last column get zeros.
+// One warp per piece: 16 rows (of one matrix, or 8 of each of two) x 128
+// columns of one expert; rows and blocks past the last get zeros.
 template <int FMT>
 __global__ void __launch_bounds__(256) k_moe_tile(const uint8_t* q, const unsigned short* d,
                                                   const uint8_t* q2, const unsigned short* d2,
@@ -1054,11 +1109,13 @@ __global__ void __launch_bounds__(256) k_moe_tile(const uint8_t* q, const unsign
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int kg = groups_of(cols), nb = cols / QK;
   const int64_t qrow = FMT == 8 ? cols : cols / 2;
-  const int tiles = q2 ? rows / 8 : rows / 16;
-  const int grp = (int)(wid % kg);
-  const int64_t tl = wid / kg, e = tl / tiles, rt = tl % tiles;
+  const int per = q2 ? 8 : 16;  // rows of each matrix in a tile
+  const int chunks = (rows + per * MOE_RT - 1) / (per * MOE_RT);
+  const int64_t ch = wid / (kg * MOE_RT), e = ch / chunks;
+  const int grp = (int)(wid / MOE_RT % kg), rt = (int)(ch % chunks) * MOE_RT + (int)(wid % MOE_RT);
+  const bool inside = rt * per < rows;  // rows are a multiple of 32: a tile is inside or past the end
   // rows g and g + 8 of the tile
-  const int64_t r0 = e * rows + (q2 ? rt * 8 + g : rt * 16 + g);
+  const int64_t r0 = e * rows + (inside ? rt * per + g : 0);
   const int64_t r1 = q2 ? r0 : r0 + 8;
   const uint8_t* qa = q + r0 * qrow;
   const uint8_t* qb = (q2 ? q2 : q) + r1 * qrow;
@@ -1071,7 +1128,7 @@ __global__ void __launch_bounds__(256) k_moe_tile(const uint8_t* q, const unsign
     const int blk = grp * 4 + b;
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[b][j] = 0u;
-    if (blk < nb) {
+    if (inside && blk < nb) {
       if (FMT == 8) {
         w[b][0] = *reinterpret_cast<const uint32_t*>(qa + blk * 32 + t * 4);
         w[b][1] = *reinterpret_cast<const uint32_t*>(qb + blk * 32 + t * 4);
@@ -1095,7 +1152,7 @@ __global__ void __launch_bounds__(256) k_moe_tile(const uint8_t* q, const unsign
   }
   // scales: [row g][block][row, row + 8]; lane (g, t) writes block t
   const int blk = grp * 4 + t;
-  const uint32_t s = blk < nb ? (uint32_t)da[blk] | (uint32_t)db[blk] << 16 : 0u;
+  const uint32_t s = inside && blk < nb ? (uint32_t)da[blk] | (uint32_t)db[blk] << 16 : 0u;
   *reinterpret_cast<uint32_t*>(o + grp_q<FMT>() + g * 16 + t * 4) = s;
 }
 
@@ -1197,10 +1254,18 @@ int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const Dev
 }
 
 template <int FMT, int DIG>
+size_t up_smem(int E, int P, int max_ent) {
+  return (size_t)ring_bytes<FMT>() + sizeof(UpPart<DIG>) + table_bytes(E, P, max_ent);
+}
+template <int FMT>
+size_t dn_smem(int E, int P, int max_ent, int N) {
+  return (size_t)ring_bytes<FMT>() + (size_t)MOE_KS * N * 16 * MOE_RT * 4 + table_bytes(E, P, max_ent);
+}
+
+template <int FMT, int DIG>
 int launch_up(const MoeArgs& a, const DeviceInfo& dev, cudaStream_t st) {
   if (int rc = allow_max_smem((const void*)k_moe_up<FMT, DIG>, dev)) return rc;
-  const size_t smem = (size_t)MOE_W * MOE_UPK * ring_bytes<FMT>() + sizeof(UpPart<DIG>) +
-                      table_bytes(a.E, a.N * a.slots, a.max_ent);
+  const size_t smem = up_smem<FMT, DIG>(a.E, a.N * a.slots, a.max_ent);
   const int64_t units = (int64_t)a.max_ent * (a.F / 32);
   const dim3 grid((unsigned)std::min<int64_t>(units, dev.sms));
   return launch("k_moe_up", k_moe_up<FMT, DIG>, grid, UP_THREADS, smem, 0, st, a);
@@ -1209,24 +1274,23 @@ int launch_up(const MoeArgs& a, const DeviceInfo& dev, cudaStream_t st) {
 template <int FMT, int DIG>
 int launch_down(const MoeArgs& a, int ydt, const DeviceInfo& dev, cudaStream_t st) {
   if (int rc = allow_max_smem((const void*)k_moe_down<FMT, DIG>, dev)) return rc;
-  const size_t smem = (size_t)MOE_W * ring_bytes<FMT>() +
-                      (size_t)a.N * 16 * MOE_W * 4 + table_bytes(a.E, a.N * a.slots, a.max_ent);
-  const int chunks = (a.K / 16 + MOE_W - 1) / MOE_W;
-  // CTAs that share 64 rows: as many as the device holds at once, four per SM
-  const int cs = std::max(1, std::min(MOE_DOWN_CL, dev.sms * 4 / chunks));
-  return launch("k_moe_down", k_moe_down<FMT, DIG>, dim3(chunks * cs), 32 * MOE_W, smem, cs, st, a, ydt);
+  const size_t smem = dn_smem<FMT>(a.E, a.N * a.slots, a.max_ent, a.N);
+  const int chunks = (a.K + 16 * MOE_RT - 1) / (16 * MOE_RT);
+  // CTAs that share 64 rows: as many as the device holds at once, one per SM
+  const int cs = std::max(1, std::min(MOE_DOWN_CL, dev.sms / chunks));
+  return launch("k_moe_down", k_moe_down<FMT, DIG>, dim3(chunks * cs), DN_THREADS, smem, cs, st, a, ydt);
 }
 
 }  // namespace
 
 size_t moe_tiles_bytes(int fmt, int64_t E, int64_t rows, int64_t cols) {
   const size_t gb = fmt == 8 ? grp_bytes<8>() : grp_bytes<4>();
-  return (size_t)E * (rows / 16) * groups_of(cols) * gb;
+  return (size_t)E * ((rows + 63) / 64 * MOE_RT) * groups_of(cols) * gb;
 }
 
 int moe_tile(int fmt, const void* q, const void* d, const void* q2, const void* d2, int64_t E,
              int64_t rows, int64_t cols, void* out, cudaStream_t st) {
-  const int64_t groups = E * (q2 ? rows / 8 : rows / 16) * groups_of(cols);
+  const int64_t groups = E * (((q2 ? 2 * rows : rows) + 63) / 64 * MOE_RT) * groups_of(cols);
   const unsigned grid = (unsigned)((groups + 7) / 8);
   auto u8 = [](const void* p) { return static_cast<const uint8_t*>(p); };
   auto u16 = [](const void* p) { return static_cast<const unsigned short*>(p); };
@@ -1282,12 +1346,20 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
   const WsMap wm = ws_map(N, slots, m.K, m.F);
   uint8_t* w = static_cast<uint8_t*>(ws);
   const int64_t xb = xdt == 0 ? 4 : 2;
-  for (int64_t n0 = 0; n0 < N; n0 += MOE_NT) {
+  // tokens of a pass: 64, or fewer where many experts or choices leave too
+  // little shared memory for the entries (1024 experts with 32 choices: 32)
+  const int et = xdt == 0 ? ent_tok<3>() : ent_tok<2>();
+  int nt = MOE_NT;
+  auto ents = [&](int n) { return std::min(m.E, n * slots) + n * slots / et; };
+  while (nt > 1 && std::max(up_smem<4, 2>(m.E, nt * slots, ents(nt)),
+                            dn_smem<4>(m.E, nt * slots, ents(nt), nt)) + 1024 > (size_t)dev.smem_optin)
+    nt /= 2;
+  for (int64_t n0 = 0; n0 < N; n0 += nt) {
     MoeArgs a = {};
     a.x = static_cast<const uint8_t*>(x) + n0 * ldx * xb;
     a.ldx = ldx;
     a.xdt = xdt;
-    a.N = (int)std::min<int64_t>(MOE_NT, N - n0);
+    a.N = (int)std::min<int64_t>(nt, N - n0);
     a.slots = slots;
     a.xdig = w + wm.xdig;
     a.xs = reinterpret_cast<float*>(w + wm.xs);
@@ -1300,9 +1372,7 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
     a.E = m.E;
     a.K = (int)m.K;
     a.F = (int)m.F;
-    // every entry but an expert's last is full
-    const int P = a.N * slots;
-    a.max_ent = std::min(m.E, P) + P / (xdt == 0 ? ent_tok<3>() : ent_tok<2>());
+    a.max_ent = ents(a.N);  // every entry but an expert's last is full
     a.y = static_cast<uint8_t*>(y) + n0 * ldy * xb;
     a.ldy = ldy;
     RouteArgs r = {};

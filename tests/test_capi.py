@@ -207,9 +207,9 @@ def test_moe_validation():
     assert rc("qgemv_moe_tile", 8, FAKE + 8, FAKE, None, None, 2, 64, 64, FAKE, None) == 3
     assert rc("qgemv_moe_tile", 4, FAKE, FAKE, None, None, 1025, 64, 64, FAKE, None) == 7
     assert rc("qgemv_moe_tile", 4, None, None, None, None, 0, 64, 64, None, None) == 0
-    # 16 rows x 128 columns: quants and 64 scales
-    assert _lib.lib().qgemv_moe_tiles_bytes(8, 3, 32, 160) == 3 * 2 * 2 * (2048 + 128)
-    assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 32, 160) == 3 * 2 * 2 * (1024 + 128)
+    # 16 rows x 128 columns: quants and 64 scales; rows padded to 64, columns to 128
+    assert _lib.lib().qgemv_moe_tiles_bytes(8, 3, 96, 160) == 3 * 8 * 2 * (2048 + 128)
+    assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 64, 160) == 3 * 4 * 2 * (1024 + 128)
     assert _lib.lib().qgemv_moe_tiles_bytes(4, 3, 40, 160) == 0
     assert _lib.lib().qgemv_moe_workspace_bytes(1, 33, 64, 64) == 0
 
