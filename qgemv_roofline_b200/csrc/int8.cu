@@ -8,13 +8,20 @@
 // is multiplied by the two scales in turn, the bias is added, and the result
 // is rounded to y's type: four roundings of an fp32 ulp's half, then y's.
 //
-// Weights take the MMA's M side (128 channels per tile), tokens its N side,
-// so that one kernel serves a single token (N = 16 columns, mostly idle: the
-// weights' stream is what counts) and a long prompt (256 tokens per tile).
+// Weights take the MMA's M side (128 channels per CTA), tokens its N side.
 // Both operands are K-major int8 rows, copied by TMA as boxes of 128 bytes
 // with 128-byte swizzle, the layout the tensor core reads; rows and columns
-// past the end read as zeros.  A CTA has a producer warp, an MMA warp and four
-// epilogue warps (one per TMEM lane quarter: lane = channel, column = token).
+// past the end read as zeros.  TMEM lane = channel, column = token: a warp
+// stores 32 consecutive channels of a token at a time.  Two kernels:
+//
+//  * k_int8_mm (few tiles): one tile of 128 channels x 16 to 128 tokens per CTA
+//    or, where there are fewer tiles than CTAs, per cluster, whose CTAs split K
+//    and add their int32 parts through distributed shared memory (exact in any
+//    order).  With one token the weights' stream is what counts.
+//  * k_int8_pair (many): persistent CTA pairs (tcgen05 cta_group::2) on tiles of
+//    256 channels x 256 tokens; each CTA copies its half of both operands, so
+//    that an SM reads 64 instead of 96 bytes of shared memory per cycle; two
+//    accumulators in TMEM, so that one tile is stored while the next is summed.
 #include <algorithm>
 #include <cstring>
 
@@ -108,13 +115,12 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
 // ---------------------------------------------------------------- product
 struct I8Args {
   alignas(64) CUtensorMap wmap;  // [M][K] int8, boxes of 128 bytes x 128 rows
-  alignas(64) CUtensorMap xmap;  // [N][K] int8, boxes of 128 bytes x BN rows
+  alignas(64) CUtensorMap xmap;  // [N][K] int8, boxes of 128 bytes x BN (pairs: 128) rows
   const float* xs;
   const float* ws;
   const float* bias;
   void* y;
   int64_t ldy;
-  int ydt;
   int M, N, nk;    // nk: K steps
   int early_w;     // the weights may be read before the dependency wait
 };
@@ -125,23 +131,52 @@ struct I8Args {
 template <int BN>
 struct I8Cfg {
   static constexpr int STAGE = I8_ABYTES + BN * I8_KB;
-  static constexpr int S = BN == 256 ? 4 : BN == 128 ? 3 : 4;
+  static constexpr int S = BN == 128 ? 3 : 4;
   static constexpr int COLS = BN < 32 ? 32 : BN;  // TMEM columns
   static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
                                     ((uint32_t)(I8_M >> 4) << 24);
   static constexpr size_t SMEM = (size_t)S * STAGE + 1024;
 };
 
-__device__ __forceinline__ void store_y(const I8Args& p, int64_t i, float v) {
-  if (p.ydt == 0) static_cast<float*>(p.y)[i] = v;
-  else if (p.ydt == 1) static_cast<__nv_bfloat16*>(p.y)[i] = __float2bfloat16(v);
-  else static_cast<__half*>(p.y)[i] = __float2half(v);
+__device__ __forceinline__ void put_y(float* y, float v) { *y = v; }
+__device__ __forceinline__ void put_y(__nv_bfloat16* y, float v) { *y = __float2bfloat16(v); }
+__device__ __forceinline__ void put_y(__half* y, float v) { *y = __float2half(v); }
+
+// NC accumulator columns (tokens) from `ta` on, this lane's channel: scaled and
+// stored; `nn` of them exist.  xs: their scales in shared memory.  y: token 0's
+// element of this channel.
+template <typename Y, int NC>
+__device__ __forceinline__ void store_cols(uint32_t ta, int nn, const float* xs, float ws, float b,
+                                           bool bias, Y* y, int64_t ldy, bool live) {
+  constexpr int STEP = NC < 32 ? 16 : 32;
+#pragma unroll 1
+  for (int c = 0; c < NC && c < nn; c += STEP) {
+    uint32_t v[STEP];
+    if constexpr (STEP == 16) tmem_ld<16>(ta + c, v);
+    else tmem_ld32(ta + c, v);
+    tmem_ld_wait();
+    if (!live) continue;
+    Y* p = y + (int64_t)c * ldy;
+    if (c + STEP <= nn) {
+#pragma unroll
+      for (int j = 0; j < STEP; ++j, p += ldy) {
+        const float f = (float)(int)v[j] * xs[c + j] * ws;
+        put_y(p, bias ? f + b : f);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < STEP; ++j, p += ldy) {
+        const float f = (float)(int)v[j] * xs[c + j] * ws;
+        if (c + j < nn) put_y(p, bias ? f + b : f);
+      }
+    }
+  }
 }
 
 // Grid (channel tiles x cluster size, token tiles).  The CTAs of a cluster
 // split the K steps of one tile; their int32 parts are added through
 // distributed shared memory (exact, so in any order).
-template <int BN>
+template <int BN, typename Y>
 __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ I8Args p) {
   using C = I8Cfg<BN>;
   constexpr int S = C::S;
@@ -149,7 +184,9 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
   __shared__ __align__(8) unsigned long long full[S], empty[S], done;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
+  __shared__ __align__(16) float xs_s[BN];
   cg::cluster_group cl = cg::this_cluster();
+  Y* y = static_cast<Y*>(p.y);
   const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   uint8_t* ring = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(i8_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -220,12 +257,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
                        db = sw128_desc(ring_s + s * C::STAGE + I8_ABYTES);
 #pragma unroll
         for (int k = 0; k < I8_KB / 32; ++k)
-          asm volatile(
-              "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-              " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem),
-              "l"(da + (uint64_t)(k * 2)), "l"(db + (uint64_t)(k * 2)), "r"(C::IDESC),
-              "r"(i > 0 || k > 0 ? 1 : 0)
-              : "memory");
+          tc_mma_i8<1>(tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), C::IDESC, i > 0 || k > 0);
         tc_commit(saddr(&empty[s]));
       }
       tc_commit(saddr(&done));
@@ -234,27 +266,26 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
   } else {
     pdl_wait();  // xs
     if (warp == 2) pdl_trigger();
+    const int nn = min(BN, p.N - n0);
+    const int quarter = warp & 3, row = quarter * 32 + lane, m = m0 + row;
+    for (int c = threadIdx.x - 64; c < nn; c += 128) xs_s[c] = p.xs[n0 + c];
+    const float ws = m < p.M ? p.ws[m] : 0.0f, b = m < p.M && p.bias ? p.bias[m] : 0.0f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
     mbar_wait(saddr(&done), 0u, &abort_flag);
     __syncwarp();
     tc_fence_after();
-    const int quarter = warp & 3, row = quarter * 32 + lane, m = m0 + row;
-    const float ws = m < p.M ? p.ws[m] : 0.0f, b = m < p.M && p.bias ? p.bias[m] : 0.0f;
     const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16);
-    int* part = reinterpret_cast<int*>(ring);  // [BN][128], once the ring is idle (done)
-    const int nn = min(BN, p.N - n0);
-    for (int c = 0; c < nn; c += 16) {
-      uint32_t v[16];
-      tmem_ld<16>(ta + c, v);
-      tmem_ld_wait();
+    if (cs > 1) {
+      int* part = reinterpret_cast<int*>(ring);  // [BN][128], once the ring is idle (done)
+      for (int c = 0; c < nn; c += 16) {
+        uint32_t v[16];
+        tmem_ld<16>(ta + c, v);
+        tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (cs > 1) {
-          part[(c + j) * I8_M + row] = (int)v[j];
-        } else if (c + j < nn && m < p.M) {
-          const float f = (float)(int)v[j] * p.xs[n0 + c + j] * ws;
-          store_y(p, (int64_t)(n0 + c + j) * p.ldy + m, p.bias ? f + b : f);
-        }
+        for (int j = 0; j < 16; ++j) part[(c + j) * I8_M + row] = (int)v[j];
       }
+    } else {
+      store_cols<Y, BN>(ta, nn, xs_s, ws, b, p.bias != nullptr, y + (int64_t)n0 * p.ldy + m, p.ldy, m < p.M);
     }
   }
   __syncwarp();
@@ -268,8 +299,8 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
         for (int c = rank; c < nn; c += cs) {
           int v = 0;
           for (int r = 0; r < cs; ++r) v += cl.map_shared_rank(part, r)[c * I8_M + row];
-          const float f = (float)v * p.xs[n0 + c] * ws;
-          store_y(p, (int64_t)(n0 + c) * p.ldy + m, p.bias ? f + b : f);
+          const float f = (float)v * xs_s[c] * ws;
+          put_y(y + (int64_t)(n0 + c) * p.ldy + m, p.bias ? f + b : f);
         }
       }
     }
@@ -282,6 +313,167 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS)
                  : "memory");
+  }
+}
+
+// ----------------------------------------------------------- CTA pairs
+constexpr int PR_N = 256;                             // tokens per tile
+constexpr int PR_STAGE = I8_ABYTES + (PR_N / 2) * I8_KB;  // a CTA's half: 32 KB
+constexpr int PR_S = 6;
+constexpr int PR_EW = 8;                              // epilogue warps
+constexpr int PR_THREADS = 32 * (2 + PR_EW);
+constexpr size_t PR_SMEM = (size_t)PR_S * PR_STAGE + 1024;
+constexpr uint32_t PR_IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PR_N >> 3) << 17) |
+                              ((uint32_t)(2 * I8_M >> 4) << 24);
+
+// Tiles t = cluster, cluster + clusters, ... of (channel tile t / token tiles,
+// token tile t % token tiles): tiles under way at the same time share channel
+// tiles, and all token tiles stay in L2.  CTA 0 of the pair issues the MMAs; the
+// copies of both CTAs complete on CTA 0's `full` barriers, and its commits
+// arrive on both CTAs' `empty` and `tfull` barriers.
+template <typename Y>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
+    k_int8_pair(const __grid_constant__ I8Args p, int ntn, int tiles) {
+  extern __shared__ uint8_t pr_smem_raw[];
+  __shared__ __align__(8) unsigned long long full[PR_S], empty[PR_S], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float xs_s[PR_EW][PR_N / 2];
+  cg::cluster_group cl = cg::this_cluster();
+  const uint32_t rank = cl.block_rank();
+  uint8_t* ring = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t ring_s = saddr(ring);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const int mine = pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0;  // tiles of this pair
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PR_S; ++s) {
+      mbar_init(saddr(&full[s]), 1);
+      mbar_init(saddr(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(saddr(&tfull[b]), 1);
+      mbar_init(saddr(&tempty[b]), 2 * PR_EW);  // both CTAs' epilogue warps
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     saddr(&tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cl.sync();  // both CTAs' barriers exist
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const int64_t total = (int64_t)mine * p.nk;
+      const uint32_t fbar = cluster_addr(saddr(&full[0]), 0);
+      auto load_w = [&](int64_t i) {
+        const int s = (int)(i % PR_S), t = pair + (int)(i / p.nk) * pairs, k = (int)(i % p.nk);
+        if (rank == 0) mbar_expect_tx(saddr(&full[s]), 2 * PR_STAGE);
+        tensor_g2s_pair(ring_s + s * PR_STAGE, &p.wmap, k * I8_KB, (t / ntn) * 2 * I8_M + (int)rank * I8_M,
+                        fbar + 8 * s);
+      };
+      auto load_x = [&](int64_t i) {
+        const int s = (int)(i % PR_S), t = pair + (int)(i / p.nk) * pairs, k = (int)(i % p.nk);
+        tensor_g2s_pair(ring_s + s * PR_STAGE + I8_ABYTES, &p.xmap, k * I8_KB,
+                        (t % ntn) * PR_N + (int)rank * (PR_N / 2), fbar + 8 * s);
+      };
+      const int pre = (int)min((int64_t)PR_S, total);
+      if (p.early_w)
+        for (int i = 0; i < pre; ++i) load_w(i);
+      pdl_wait();
+      if (!p.early_w)
+        for (int i = 0; i < pre; ++i) load_w(i);
+      for (int i = 0; i < pre; ++i) load_x(i);
+      int64_t issued = pre;
+      for (int64_t i = pre; i < total; ++i) {
+        if (!mbar_wait(saddr(&empty[i % PR_S]), (uint32_t)((i / PR_S - 1) & 1), &abort_flag)) break;
+        load_w(i);
+        load_x(i);
+        issued = i + 1;
+      }
+      // no copy outlives the pair (CTA 1's complete on CTA 0's barriers; the
+      // cluster barrier below holds CTA 1 until CTA 0 has seen them)
+      if (rank == 0)
+        for (int64_t i = max((int64_t)0, issued - PR_S); i < issued; ++i)
+          mbar_wait_drain(saddr(&full[i % PR_S]), (uint32_t)((i / PR_S) & 1));
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (lane == 0 && rank == 0) {
+      pdl_wait();  // so that the bounded waits below do not count the previous kernel's time
+      bool ok = true;
+      int64_t i = 0;
+      int t = 0;
+      for (; t < mine && ok; ++t) {
+        const int b = t & 1;
+        if (t >= 2) ok = mbar_wait(saddr(&tempty[b]), (uint32_t)((t / 2 - 1) & 1), &abort_flag);
+        tc_fence_after();
+        for (int k = 0; k < p.nk && ok; ++k, ++i) {
+          const int s = (int)(i % PR_S);
+          ok = mbar_wait(saddr(&full[s]), (uint32_t)((i / PR_S) & 1), &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = sw128_desc(ring_s + s * PR_STAGE), db = sw128_desc(ring_s + s * PR_STAGE + I8_ABYTES);
+#pragma unroll
+          for (int kk = 0; kk < I8_KB / 32; ++kk)
+            tc_mma_i8<2>(tmem + b * PR_N, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), PR_IDESC,
+                         k > 0 || kk > 0);
+          tc_commit_pair(saddr(&empty[s]));
+        }
+        if (ok) tc_commit_pair(saddr(&tfull[b]));
+      }
+      // no MMA outlives the pair's operands or accumulators: the last commit
+      if (ok && mine > 0) mbar_wait_drain(saddr(&tfull[(mine - 1) & 1]), (uint32_t)(((mine - 1) / 2) & 1));
+      else if (!ok) {
+        tc_commit_pair(saddr(&tfull[t & 1]));
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {  // a launch that gave up: what was issued ends within microseconds
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    pdl_wait();
+    if (warp == 2) pdl_trigger();
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    float* xs = xs_s[warp - 2];
+    for (int t = 0; t < mine; ++t) {
+      const int tile = pair + t * pairs, b = t & 1;
+      const int m = (tile / ntn) * 2 * I8_M + (int)rank * I8_M + quarter * 32 + lane;
+      const int n0 = (tile % ntn) * PR_N + half * (PR_N / 2), nn = min(PR_N / 2, p.N - n0);
+      __syncwarp();
+      for (int c = lane; c < nn; c += 32) xs[c] = p.xs[n0 + c];
+      const float ws = m < p.M ? p.ws[m] : 0.0f, bv = m < p.M && p.bias ? p.bias[m] : 0.0f;
+      __syncwarp();
+      if (!mbar_wait(saddr(&tfull[b]), (uint32_t)((t / 2) & 1), &abort_flag)) break;
+      __syncwarp();
+      tc_fence_after();
+      store_cols<Y, PR_N / 2>(tmem + ((uint32_t)(quarter * 32) << 16) + b * PR_N + half * (PR_N / 2), nn, xs, ws, bv,
+                              p.bias != nullptr, static_cast<Y*>(p.y) + (int64_t)n0 * p.ldy + m, p.ldy, m < p.M);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(saddr(&tempty[b]), 0));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cl.sync();  // neither CTA leaves while the pair's copies, MMAs or arrivals reach it
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
@@ -301,7 +493,7 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, f, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -310,10 +502,10 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
   return OK;
 }
 
-template <int BN>
+template <int BN, typename Y>
 int launch_mm(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t st) {
   using C = I8Cfg<BN>;
-  if (int rc = allow_max_smem((const void*)k_int8_mm<BN>, dev)) return rc;
+  if (int rc = allow_max_smem((const void*)k_int8_mm<BN, Y>, dev)) return rc;
   const int tiles = (int)((c.M + I8_M - 1) / I8_M);
   const int64_t step = (int64_t)BN * 65535;  // token tiles of one launch
   for (int64_t n0 = 0; n0 < c.N; n0 += step) {
@@ -324,17 +516,52 @@ int launch_mm(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
                                   c.ldx, I8_KB, BN, true))
       return rc;
     a.xs = c.xs + n0;
-    a.y = static_cast<uint8_t*>(c.y) + n0 * c.ldy * (c.ydt == 0 ? 4 : 2);
+    a.y = static_cast<Y*>(c.y) + n0 * c.ldy;
     a.N = (int)n;
     // few tiles: a cluster splits the K steps, as many CTAs as fit at once
     const int per_sm = std::max(1, (int)((size_t)dev.smem_optin / C::SMEM));
     int cs = 1;
     while (cs < 8 && tiles * nt * cs * 2 <= (int64_t)per_sm * dev.sms && a.nk >= cs * 4) cs *= 2;
-    if (int rc = launch("k_int8_mm", k_int8_mm<BN>, dim3(tiles * cs, (unsigned)nt), I8_THREADS, C::SMEM,
+    if (int rc = launch("k_int8_mm", k_int8_mm<BN, Y>, dim3(tiles * cs, (unsigned)nt), I8_THREADS, C::SMEM,
                         cs, st, a))
       return rc;
   }
   return OK;
+}
+
+template <typename Y>
+int launch_pair(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t st) {
+  if (int rc = allow_max_smem((const void*)k_int8_pair<Y>, dev)) return rc;
+  const int64_t mt = (c.M + 2 * I8_M - 1) / (2 * I8_M);
+  const int64_t step = std::max<int64_t>(1, (((int64_t)1 << 30) / mt)) * PR_N;  // tiles of one launch below 2^30
+  for (int64_t n0 = 0; n0 < c.N; n0 += step) {
+    const int64_t n = std::min(step, c.N - n0), ntn = (n + PR_N - 1) / PR_N;
+    if (int rc = encode_tensor_2d(&a.wmap, false, c.wq, c.K, c.M, c.ldw, I8_KB, I8_M, true)) return rc;
+    if (int rc = encode_tensor_2d(&a.xmap, false, static_cast<const int8_t*>(c.xq) + n0 * c.ldx, c.K, n,
+                                  c.ldx, I8_KB, PR_N / 2, true))
+      return rc;
+    a.xs = c.xs + n0;
+    a.y = static_cast<Y*>(c.y) + n0 * c.ldy;
+    a.N = (int)n;
+    const int64_t tiles = mt * ntn;
+    const int pairs = (int)std::min<int64_t>(tiles, dev.sms / 2);
+    // the cluster size is the kernel's own
+    if (int rc = launch("k_int8_pair", k_int8_pair<Y>, dim3(2 * pairs), PR_THREADS, PR_SMEM, 0, st, a, (int)ntn,
+                        (int)tiles))
+      return rc;
+  }
+  return OK;
+}
+
+template <typename Y>
+int matmul_as(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t st) {
+  if (c.N <= 16) return launch_mm<16, Y>(c, a, dev, st);
+  if (c.N <= 32) return launch_mm<32, Y>(c, a, dev, st);
+  if (c.N <= 64) return launch_mm<64, Y>(c, a, dev, st);
+  // pairs where their tiles fill the device, else tiles of 128 x 128
+  const int64_t tiles = ((c.M + 2 * I8_M - 1) / (2 * I8_M)) * ((c.N + PR_N - 1) / PR_N);
+  if (tiles < dev.sms / 2) return launch_mm<128, Y>(c, a, dev, st);
+  return launch_pair<Y>(c, a, dev, st);
 }
 
 }  // namespace
@@ -369,15 +596,12 @@ int int8_matmul(const Int8Call& c, bool early_w, cudaStream_t st) {
   a.ws = c.ws;
   a.bias = c.bias;
   a.ldy = c.ldy;
-  a.ydt = c.ydt;
   a.M = (int)c.M;
   a.nk = (int)((c.K + I8_KB - 1) / I8_KB);
   a.early_w = early_w;
-  if (c.N <= 16) return launch_mm<16>(c, a, dev, st);
-  if (c.N <= 32) return launch_mm<32>(c, a, dev, st);
-  if (c.N <= 64) return launch_mm<64>(c, a, dev, st);
-  if (c.N <= 128) return launch_mm<128>(c, a, dev, st);
-  return launch_mm<256>(c, a, dev, st);
+  if (c.ydt == 0) return matmul_as<float>(c, a, dev, st);
+  if (c.ydt == 1) return matmul_as<__nv_bfloat16>(c, a, dev, st);
+  return matmul_as<__half>(c, a, dev, st);
 }
 
 int set_i8_spin_limit(long long cycles) {
