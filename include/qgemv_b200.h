@@ -600,7 +600,8 @@ QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_r
  * y[n][m] = (sum_k xq[n][k] wq[m][k]) * xs[n] * ws[m] (+ bias[m])
  * with int8 rows and one fp32 scale per token n and per channel m, any number
  * of tokens.  The sum is exact (int32); it is rounded to fp32, multiplied by
- * xs, then by ws, the bias is added, and the result is rounded to y's type
+ * xs, then by ws with the bias added (one fused operation), and the result is
+ * rounded to y's type
  * (QGEMV_F32, QGEMV_BF16 or QGEMV_F16).  K % 16 == 0, 16 <= K < 2^17; xq and
  * wq 16-byte aligned with row strides (in bytes) that are multiples of 16.
  * Row n of y is at y + n * ldy elements.

@@ -1072,7 +1072,7 @@ QGEMV_API int qgemv_int8_quantize(const void* x, int dtype, int64_t ldx, int64_t
   if (rows > 1 && (ldx < K || ldq < K))
     return set_error(ERR_SHAPE, "ldx=%lld and ldq=%lld must be at least K=%lld", (long long)ldx,
                      (long long)ldq, (long long)K);
-  return int8_quantize(x, dtype, ldx, rows, K, q, ldq, K, scales, static_cast<cudaStream_t>(stream));
+  return int8_quantize(x, dtype, ldx, rows, K, q, ldq, scales, static_cast<cudaStream_t>(stream));
 }
 
 QGEMV_API int qgemv_int8_matmul(const void* xq, const float* xs, int64_t ldx, const void* wq,
@@ -1114,7 +1114,7 @@ QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const voi
   }
   float* xs = static_cast<float*>(workspace);
   void* xq = static_cast<uint8_t*>(workspace) + (size_t)((N + 31) / 32 * 32) * 4;
-  if (int rc = int8_quantize(x, dtype, ldx, N, K, xq, K, K, xs, st)) return rc;
+  if (int rc = int8_quantize(x, dtype, ldx, N, K, xq, K, xs, st)) return rc;
   return int8_entry(xq, xs, K, wq, ws, ldw, bias, N, M, K, y, y_dtype, ldy, true, stream);
 }
 

@@ -5,8 +5,9 @@
 //
 // The sum is exact: tcgen05.mma kind::i8 accumulates in int32, which holds
 // K * 128 * 128 for K below 2^17 (larger K is refused).  It becomes fp32 once,
-// is multiplied by the two scales in turn, the bias is added, and the result
-// is rounded to y's type: four roundings of an fp32 ulp's half, then y's.
+// is multiplied by the token's scale, then by the channel's with the bias added
+// in the same operation, and the result is rounded to y's type: three roundings
+// to fp32, then y's.
 //
 // Weights take the MMA's M side (128 channels per CTA), tokens its N side.
 // Both operands are K-major int8 rows, copied by TMA as boxes of 128 bytes
@@ -77,20 +78,27 @@ template <typename T> __device__ __forceinline__ float as_f32(T v) { return (flo
 template <> __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ int8_t quant1(float v, float s) {
-  // IEEE division: the rounding of x / s is the definition's
-  const float r = rintf(__fdiv_rn(v, s));
-  return (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
+// rint(x / s), the quotient rounded to fp32 first.  x * (1 / s) is within
+// 127 * 2^-22 of it, so only quotients that near to a tie (or any, where 1 / s
+// is not accurate) need the division itself.
+__device__ __forceinline__ int quant1(float v, float s, float inv, bool exact) {
+  const float r = v * inv;
+  float q = rintf(r);
+  if (exact || fabsf(fabsf(r - q) - 0.5f) < 6.2e-5f)
+    q = fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
+  return (int)q;
 }
 
 constexpr int RQ_THREADS = 256;
+constexpr int RQ_HELD = 4;  // vectors of 8 values that a thread keeps
 
 // One CTA per row.  A row with a NaN or an infinity gets the scale NaN and
 // zeros; an all-zero row (or one whose scale underflows to 0) the scale 0 and
-// zeros.  Columns [K, kpad) get zeros.
-template <typename T>
+// zeros.  VEC: rows start on 16-byte boundaries, q's on 8-byte ones, and K is a
+// multiple of 8: a row of up to 8192 values is read once and kept.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__ x, int64_t ldx, int K,
-                                                           int8_t* __restrict__ q, int64_t ldq, int kpad,
+                                                           int8_t* __restrict__ q, int64_t ldq,
                                                            float* __restrict__ s) {
   __shared__ uint32_t red[RQ_THREADS / 32];
   pdl_wait();
@@ -98,8 +106,40 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
   int8_t* qr = q + row * ldq;
+  auto load8 = [&](float (&v)[8], int i) {  // values 8 i ...
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(xr)[2 * i], b = reinterpret_cast<const float4*>(xr)[2 * i + 1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 a = reinterpret_cast<const uint4*>(xr)[i];
+      const T* t = reinterpret_cast<const T*>(&a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = as_f32(t[j]);
+    }
+  };
+  auto bits = [](float v) { return __float_as_uint(v) & 0x7FFFFFFFu; };
   uint32_t m = 0u;
-  for (int k = threadIdx.x; k < K; k += RQ_THREADS) m = max(m, __float_as_uint(as_f32(xr[k])) & 0x7FFFFFFFu);
+  float held[RQ_HELD][8];
+  const int nv = K / 8;
+  if (VEC) {
+#pragma unroll
+    for (int h = 0; h < RQ_HELD; ++h) {
+      const int i = threadIdx.x + h * RQ_THREADS;
+      if (i < nv) {
+        load8(held[h], i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, bits(held[h][j]));
+      }
+    }
+    for (int i = threadIdx.x + RQ_HELD * RQ_THREADS; i < nv; i += RQ_THREADS) {
+      float v[8];
+      load8(v, i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, bits(v[j]));
+    }
+  } else {
+    for (int k = threadIdx.x; k < K; k += RQ_THREADS) m = max(m, bits(as_f32(xr[k])));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
@@ -107,9 +147,32 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
   for (int i = 0; i < RQ_THREADS / 32; ++i) m = max(m, red[i]);
   const bool bad = m >= 0x7F800000u;
   const float sc = bad ? __int_as_float(0x7FC00000) : __fdiv_rn(__uint_as_float(m), 127.0f);
-  for (int k = threadIdx.x; k < kpad; k += RQ_THREADS)
-    qr[k] = k < K && sc > 0.0f ? quant1(as_f32(xr[k]), sc) : (int8_t)0;
+  const bool some = sc > 0.0f, exact = sc < 7.9e-31f;  // 2^-100: 1 / s stays a normal number above
+  const float inv = some ? __fdiv_rn(1.0f, sc) : 0.0f;
   if (threadIdx.x == 0) s[row] = sc;
+  if (VEC) {
+    auto put8 = [&](const float (&v)[8], int i) {
+      uint32_t w[2] = {0u, 0u};
+      if (some) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(quant1(v[j], sc, inv, exact) & 0xFF) << (8 * (j & 3));
+      }
+      reinterpret_cast<uint2*>(qr)[i] = make_uint2(w[0], w[1]);
+    };
+#pragma unroll
+    for (int h = 0; h < RQ_HELD; ++h) {
+      const int i = threadIdx.x + h * RQ_THREADS;
+      if (i < nv) put8(held[h], i);
+    }
+    for (int i = threadIdx.x + RQ_HELD * RQ_THREADS; i < nv; i += RQ_THREADS) {
+      float v[8];
+      load8(v, i);
+      put8(v, i);
+    }
+  } else {
+    for (int k = threadIdx.x; k < K; k += RQ_THREADS)
+      qr[k] = some ? (int8_t)quant1(as_f32(xr[k]), sc, inv, exact) : (int8_t)0;
+  }
 }
 
 // ---------------------------------------------------------------- product
@@ -141,34 +204,53 @@ struct I8Cfg {
 __device__ __forceinline__ void put_y(float* y, float v) { *y = v; }
 __device__ __forceinline__ void put_y(__nv_bfloat16* y, float v) { *y = __float2bfloat16(v); }
 __device__ __forceinline__ void put_y(__half* y, float v) { *y = __float2half(v); }
+// two channels of one token
+__device__ __forceinline__ void put_y2(__nv_bfloat16* y, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(y) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void put_y2(__half* y, float a, float b) {
+  *reinterpret_cast<__half2*>(y) = __floats2half2_rn(a, b);
+}
 
 // NC accumulator columns (tokens) from `ta` on, this lane's channel: scaled and
 // stored; `nn` of them exist.  xs: their scales in shared memory.  y: token 0's
-// element of this channel.
+// element of the warp's first channel; `room`: channels from there on.  With a
+// 16-bit type and even addresses a pair of lanes trades values, so that one
+// store writes two channels of one token in the even lane and of the next in the
+// odd one (4096 tokens, 4096 -> 22016: the stores, not the MMAs, set the pace at
+// one value a store).
 template <typename Y, int NC>
-__device__ __forceinline__ void store_cols(uint32_t ta, int nn, const float* xs, float ws, float b,
-                                           bool bias, Y* y, int64_t ldy, bool live) {
+__device__ __forceinline__ void store_cols(uint32_t ta, int nn, const float* xs, float ws, float b, Y* y,
+                                           int64_t ldy, int room, int lane) {
   constexpr int STEP = NC < 32 ? 16 : 32;
+  const bool pairs = sizeof(Y) == 2 && room >= 32 && (reinterpret_cast<uintptr_t>(y) & 3) == 0 && (ldy & 1) == 0;
+  const bool odd = lane & 1;
 #pragma unroll 1
   for (int c = 0; c < NC && c < nn; c += STEP) {
     uint32_t v[STEP];
     if constexpr (STEP == 16) tmem_ld<16>(ta + c, v);
     else tmem_ld32(ta + c, v);
     tmem_ld_wait();
-    if (!live) continue;
     Y* p = y + (int64_t)c * ldy;
-    if (c + STEP <= nn) {
+    if (sizeof(Y) == 2 && pairs && c + STEP <= nn) {
+      if constexpr (sizeof(Y) == 2) {
+        p += (lane & ~1) + (odd ? ldy : 0);
 #pragma unroll
-      for (int j = 0; j < STEP; ++j, p += ldy) {
-        const float f = (float)(int)v[j] * xs[c + j] * ws;
-        put_y(p, bias ? f + b : f);
+        for (int j = 0; j < STEP; j += 4, p += 4 * ldy) {
+          const float4 s = *reinterpret_cast<const float4*>(xs + c + j);
+          const float f0 = fmaf((float)(int)v[j] * s.x, ws, b), f1 = fmaf((float)(int)v[j + 1] * s.y, ws, b);
+          const float f2 = fmaf((float)(int)v[j + 2] * s.z, ws, b), f3 = fmaf((float)(int)v[j + 3] * s.w, ws, b);
+          const float g = __shfl_xor_sync(0xffffffffu, odd ? f0 : f1, 1);
+          const float h = __shfl_xor_sync(0xffffffffu, odd ? f2 : f3, 1);
+          put_y2(p, odd ? g : f0, odd ? f1 : g);
+          put_y2(p + 2 * ldy, odd ? h : f2, odd ? f3 : h);
+        }
       }
     } else {
+      p += lane;
 #pragma unroll
-      for (int j = 0; j < STEP; ++j, p += ldy) {
-        const float f = (float)(int)v[j] * xs[c + j] * ws;
-        if (c + j < nn) put_y(p, bias ? f + b : f);
-      }
+      for (int j = 0; j < STEP; ++j, p += ldy)
+        if (c + j < nn && lane < room) put_y(p, fmaf((float)(int)v[j] * xs[c + j], ws, b));
     }
   }
 }
@@ -285,7 +367,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
         for (int j = 0; j < 16; ++j) part[(c + j) * I8_M + row] = (int)v[j];
       }
     } else {
-      store_cols<Y, BN>(ta, nn, xs_s, ws, b, p.bias != nullptr, y + (int64_t)n0 * p.ldy + m, p.ldy, m < p.M);
+      store_cols<Y, BN>(ta, nn, xs_s, ws, b, y + (int64_t)n0 * p.ldy + m - lane, p.ldy, p.M - m + lane, lane);
     }
   }
   __syncwarp();
@@ -299,8 +381,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
         for (int c = rank; c < nn; c += cs) {
           int v = 0;
           for (int r = 0; r < cs; ++r) v += cl.map_shared_rank(part, r)[c * I8_M + row];
-          const float f = (float)v * xs_s[c] * ws;
-          put_y(y + (int64_t)(n0 + c) * p.ldy + m, p.bias ? f + b : f);
+          put_y(y + (int64_t)(n0 + c) * p.ldy + m, fmaf((float)v * xs_s[c], ws, b));
         }
       }
     }
@@ -375,32 +456,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const int64_t total = (int64_t)mine * p.nk;
+      // a step at a time: K step k of tile t into stage s (counted, not divided:
+      // one thread does all this, in the time of four MMAs)
+      struct At {
+        int s, k, t;
+      };
       const uint32_t fbar = cluster_addr(saddr(&full[0]), 0);
-      auto load_w = [&](int64_t i) {
-        const int s = (int)(i % PR_S), t = pair + (int)(i / p.nk) * pairs, k = (int)(i % p.nk);
-        if (rank == 0) mbar_expect_tx(saddr(&full[s]), 2 * PR_STAGE);
-        tensor_g2s_pair(ring_s + s * PR_STAGE, &p.wmap, k * I8_KB, (t / ntn) * 2 * I8_M + (int)rank * I8_M,
-                        fbar + 8 * s);
+      auto next = [&](At& at) {
+        if (++at.s == PR_S) at.s = 0;
+        if (++at.k == p.nk) {
+          at.k = 0;
+          at.t += pairs;
+        }
       };
-      auto load_x = [&](int64_t i) {
-        const int s = (int)(i % PR_S), t = pair + (int)(i / p.nk) * pairs, k = (int)(i % p.nk);
-        tensor_g2s_pair(ring_s + s * PR_STAGE + I8_ABYTES, &p.xmap, k * I8_KB,
-                        (t % ntn) * PR_N + (int)rank * (PR_N / 2), fbar + 8 * s);
+      auto load_w = [&](const At& at, int m0) {
+        if (rank == 0) mbar_expect_tx(saddr(&full[at.s]), 2 * PR_STAGE);
+        tensor_g2s_pair(ring_s + at.s * PR_STAGE, &p.wmap, at.k * I8_KB, m0, fbar + 8 * at.s);
       };
+      auto load_x = [&](const At& at, int n0) {
+        tensor_g2s_pair(ring_s + at.s * PR_STAGE + I8_ABYTES, &p.xmap, at.k * I8_KB, n0, fbar + 8 * at.s);
+      };
+      auto m_of = [&](int t) { return (t / ntn) * 2 * I8_M + (int)rank * I8_M; };
+      auto n_of = [&](int t) { return (t % ntn) * PR_N + (int)rank * (PR_N / 2); };
+      const int64_t total = (int64_t)mine * p.nk;
       const int pre = (int)min((int64_t)PR_S, total);
+      At at{0, 0, pair};
       if (p.early_w)
-        for (int i = 0; i < pre; ++i) load_w(i);
+        for (int i = 0; i < pre; ++i, next(at)) load_w(at, m_of(at.t));
       pdl_wait();
-      if (!p.early_w)
-        for (int i = 0; i < pre; ++i) load_w(i);
-      for (int i = 0; i < pre; ++i) load_x(i);
+      at = At{0, 0, pair};
+      for (int i = 0; i < pre; ++i, next(at)) {
+        if (!p.early_w) load_w(at, m_of(at.t));
+        load_x(at, n_of(at.t));
+      }
       int64_t issued = pre;
-      for (int64_t i = pre; i < total; ++i) {
-        if (!mbar_wait(saddr(&empty[i % PR_S]), (uint32_t)((i / PR_S - 1) & 1), &abort_flag)) break;
-        load_w(i);
-        load_x(i);
-        issued = i + 1;
+      uint32_t phase = 0u;
+      int m0 = m_of(at.t), n0 = n_of(at.t);
+      while (issued < total) {
+        if (!mbar_wait(saddr(&empty[at.s]), phase, &abort_flag)) break;
+        if (at.k == 0) {
+          m0 = m_of(at.t);
+          n0 = n_of(at.t);
+        }
+        load_w(at, m0);
+        load_x(at, n0);
+        next(at);
+        if (at.s == 0) phase ^= 1u;
+        ++issued;
       }
       // no copy outlives the pair (CTA 1's complete on CTA 0's barriers; the
       // cluster barrier below holds CTA 1 until CTA 0 has seen them)
@@ -413,15 +515,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
     if (lane == 0 && rank == 0) {
       pdl_wait();  // so that the bounded waits below do not count the previous kernel's time
       bool ok = true;
-      int64_t i = 0;
-      int t = 0;
+      int s = 0, t = 0;
+      uint32_t phase = 0u;
       for (; t < mine && ok; ++t) {
         const int b = t & 1;
         if (t >= 2) ok = mbar_wait(saddr(&tempty[b]), (uint32_t)((t / 2 - 1) & 1), &abort_flag);
         tc_fence_after();
-        for (int k = 0; k < p.nk && ok; ++k, ++i) {
-          const int s = (int)(i % PR_S);
-          ok = mbar_wait(saddr(&full[s]), (uint32_t)((i / PR_S) & 1), &abort_flag);
+        for (int k = 0; k < p.nk && ok; ++k) {
+          ok = mbar_wait(saddr(&full[s]), phase, &abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint64_t da = sw128_desc(ring_s + s * PR_STAGE), db = sw128_desc(ring_s + s * PR_STAGE + I8_ABYTES);
@@ -430,6 +531,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
             tc_mma_i8<2>(tmem + b * PR_N, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), PR_IDESC,
                          k > 0 || kk > 0);
           tc_commit_pair(saddr(&empty[s]));
+          if (++s == PR_S) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
         if (ok) tc_commit_pair(saddr(&tfull[b]));
       }
@@ -460,7 +565,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       __syncwarp();
       tc_fence_after();
       store_cols<Y, PR_N / 2>(tmem + ((uint32_t)(quarter * 32) << 16) + b * PR_N + half * (PR_N / 2), nn, xs, ws, bv,
-                              p.bias != nullptr, static_cast<Y*>(p.y) + (int64_t)n0 * p.ldy + m, p.ldy, m < p.M);
+                              static_cast<Y*>(p.y) + (int64_t)n0 * p.ldy + m - lane, p.ldy, p.M - m + lane, lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(cluster_addr(saddr(&tempty[b]), 0));
@@ -566,26 +671,28 @@ int matmul_as(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
 
 }  // namespace
 
-int int8_quantize(const void* x, int xdt, int64_t ldx, int64_t N, int64_t K, void* q, int64_t ldq,
-                  int64_t kpad, float* s, cudaStream_t st) {
-  int8_t* qq = static_cast<int8_t*>(q);
+namespace {
+template <typename T>
+int quantize_as(const T* x, int64_t ldx, int64_t N, int64_t K, int8_t* q, int64_t ldq, float* s, cudaStream_t st) {
+  const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0 &&
+                   (N == 1 || (ldx * (int64_t)sizeof(T) % 16 == 0 && ldq % 8 == 0));
   constexpr int64_t kStep = (int64_t)1 << 30;  // rows of one launch
   for (int64_t n0 = 0; n0 < N; n0 += kStep) {
     const dim3 grid((unsigned)std::min(kStep, N - n0));
-    int rc;
-    if (xdt == 0)
-      rc = launch("k_quant_rows", k_quant_rows<float>, grid, RQ_THREADS, 0, 1, st,
-                  static_cast<const float*>(x) + n0 * ldx, ldx, (int)K, qq + n0 * ldq, ldq, (int)kpad, s + n0);
-    else if (xdt == 1)
-      rc = launch("k_quant_rows", k_quant_rows<__nv_bfloat16>, grid, RQ_THREADS, 0, 1, st,
-                  static_cast<const __nv_bfloat16*>(x) + n0 * ldx, ldx, (int)K, qq + n0 * ldq, ldq,
-                  (int)kpad, s + n0);
-    else
-      rc = launch("k_quant_rows", k_quant_rows<__half>, grid, RQ_THREADS, 0, 1, st,
-                  static_cast<const __half*>(x) + n0 * ldx, ldx, (int)K, qq + n0 * ldq, ldq, (int)kpad, s + n0);
-    if (rc) return rc;
+    if (int rc = launch("k_quant_rows", vec ? k_quant_rows<T, true> : k_quant_rows<T, false>, grid, RQ_THREADS, 0, 0,
+                        st, x + n0 * ldx, ldx, (int)K, q + n0 * ldq, ldq, s + n0))
+      return rc;
   }
   return OK;
+}
+}  // namespace
+
+int int8_quantize(const void* x, int xdt, int64_t ldx, int64_t N, int64_t K, void* q, int64_t ldq, float* s,
+                  cudaStream_t st) {
+  int8_t* qq = static_cast<int8_t*>(q);
+  if (xdt == 0) return quantize_as(static_cast<const float*>(x), ldx, N, K, qq, ldq, s, st);
+  if (xdt == 1) return quantize_as(static_cast<const __nv_bfloat16*>(x), ldx, N, K, qq, ldq, s, st);
+  return quantize_as(static_cast<const __half*>(x), ldx, N, K, qq, ldq, s, st);
 }
 
 int int8_matmul(const Int8Call& c, bool early_w, cudaStream_t st) {

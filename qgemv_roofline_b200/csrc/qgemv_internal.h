@@ -215,7 +215,7 @@ struct Int8Call {
   int ydt = 0;
 };
 int int8_quantize(const void* x, int xdt, int64_t ldx, int64_t N, int64_t K, void* q, int64_t ldq,
-                  int64_t kpad, float* s, cudaStream_t st);
+                  float* s, cudaStream_t st);
 // early_w: the launch before this one was int8_quantize's on the same stream
 // (the weights may be read before it has finished).
 int int8_matmul(const Int8Call& c, bool early_w, cudaStream_t st);
