@@ -57,8 +57,10 @@
 // into the high half of a byte is 16 (n - 8) as a signed byte, one or two
 // instructions; the 1/16 is folded into the result's factor (exact).
 #include <algorithm>
+#include <map>
 #include <mutex>
 #include <set>
+#include <tuple>
 #include <utility>
 
 #include <cooperative_groups.h>
@@ -240,15 +242,46 @@ constexpr int RT_TE = 4;    // experts of a warp's tile
 // x columns staged at a time, as doubles (32 KB)
 template <int TN> __host__ __device__ constexpr int rt_chunk() { return TN == 1 ? 4096 : TN == 2 ? 2048 : 512; }
 
-// Ordering key of a score: larger key = larger score; NaN lowest; +0 == -0.
+// Ordering keys of a score: larger key = larger score, +0 == -0, NaN lowest (1;
+// 0 marks a taken expert).
 __device__ __forceinline__ unsigned long long rank_key(double v) {
-  if (v != v) return 0ull;
+  if (v != v) return 1ull;
   const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
-
-__device__ __forceinline__ double load_as_f64(const void* p, int dt, int64_t i) {
-  return (double)load_as_f32(p, dt, i);
+__device__ __forceinline__ uint32_t rank_key(float v) {
+  if (v != v) return 1u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+// The largest key of the warp's lanes.
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
+  const uint32_t hi = (uint32_t)(k >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
+  const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? (uint32_t)k : 0u);
+  return (unsigned long long)mh << 32 | ml;
+}
+// k rounds over E keys in shared memory; lane j returns the j-th choice.  Lane
+// l's experts are l, l + 32, ...; equal keys go to the lowest expert.
+template <typename Key>
+__device__ __forceinline__ int pick(Key* key, int E, int k, int lane) {
+  int mine = 0;
+  for (int j = 0; j < k; ++j) {
+    Key best = 0;
+    int at = lane;
+#pragma unroll 4
+    for (int e = lane; e < E; e += 32)
+      if (key[e] > best) {
+        best = key[e];
+        at = e;
+      }
+    const Key top = warp_max(best);
+    const int win = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)at : 0xFFFFFFFFu);
+    if (lane == j) mine = win;
+    if (win == at) key[win] = 0;
+    __syncwarp();
+  }
+  return mine;
 }
 
 // Four consecutive values from element i on as fp32, those past `n` zero; one
@@ -274,69 +307,41 @@ __device__ __forceinline__ void load4(float (&v)[4], const void* p, int dt, int6
   }
 }
 
-// The top k of one token by one warp: `logit` and `key` hold E values in
-// shared memory.  Ties go to the lowest index.
-__device__ void route_token(const RouteArgs& r, const float* logit, unsigned long long* key,
-                            int n, int lane) {
-  const int E = r.E;
-  // statistics in 32 bits: max, sum of exp over all experts, any NaN
+// The top k of one token by one warp: `logit` holds E values in shared memory,
+// `key` room for as many 64-bit keys.  (A token's choice is latency and little
+// else, run once per launch from a cold instruction cache: short loops.)
+__device__ void route_token(const RouteArgs& r, const float* logit, unsigned long long* key, int n, int lane) {
+  const int E = r.E, slots = r.k + r.shared;
+  uint32_t* key32 = reinterpret_cast<uint32_t*>(key);
   float mx = -INFINITY;
   bool nan = false;
   for (int e = lane; e < E; e += 32) {
-    mx = fmaxf(mx, logit[e]);
-    nan |= logit[e] != logit[e];
+    const float l = logit[e];
+    mx = fmaxf(mx, l);
+    nan |= l != l;
+    key32[e] = rank_key(l);
   }
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   nan = __any_sync(0xffffffffu, nan);
-  float all = 0.0f;
-  double all64 = 0.0;
-  if (r.scoring == 0) {
-    for (int e = lane; e < E; e += 32) all += expf(logit[e] - mx);
-    all = warp_sum(all);
-    if (r.bias) {
-      for (int e = lane; e < E; e += 32) all64 += exp((double)logit[e] - (double)mx);
-      for (int o = 16; o; o >>= 1) all64 += __shfl_xor_sync(0xffffffffu, all64, o);
-    }
-  }
-  // softmax and sigmoid are increasing, so without a bias the logits rank the
-  // experts; with one the scores are formed in 64 bits, so that rounding does
-  // not decide between near scores
-  for (int e = lane; e < E; e += 32) {
-    double v = (double)logit[e];
-    if (r.bias)
-      v = (r.scoring == 0 ? exp(v - (double)mx) / all64 : 1.0 / (1.0 + exp(-v))) + (double)r.bias[e];
-    key[e] = rank_key(v);
-  }
   __syncwarp();
-  // each lane's best of its own experts (e = lane, lane + 32, ...); after a
-  // round only the winner's lane looks again.  A taken expert is marked by
-  // its bit (experts of a lane: at most 32).
-  uint32_t taken = 0u;
-  unsigned long long best = 0ull;
-  int at = -1;
-  auto look = [&]() {
-    at = -1;
-    best = 0ull;
-    for (int i = 0, e = lane; e < E; ++i, e += 32)
-      if (!((taken >> i) & 1u) && (at < 0 || key[e] > best)) {
-        best = key[e];
-        at = e;
-      }
-  };
-  look();
-  const int slots = r.k + r.shared;
-  int mine = -1;  // lane j keeps the j-th choice
-  for (int j = 0; j < r.k; ++j) {
-    const uint32_t hi = at < 0 ? 0u : (uint32_t)(best >> 32), lo = at < 0 ? 0u : (uint32_t)best;
-    const uint32_t mh = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? lo : 0u);
-    const int win = (int)__reduce_min_sync(
-        0xffffffffu, at >= 0 && hi == mh && lo == ml ? (uint32_t)at : 0xFFFFFFFFu);
-    if (lane == j) mine = win;
-    if (win == at) {
-      taken |= 1u << (win >> 5);
-      look();
+  int mine;
+  if (!r.bias) {
+    // softmax and sigmoid are increasing: the logits rank the experts
+    mine = pick(key32, E, r.k, lane);
+  } else {
+    // with a bias the scores are formed in 64 bits, so that rounding does not
+    // decide between near scores
+    double all = 0.0;
+    if (r.scoring == 0) {
+      for (int e = lane; e < E; e += 32) all += exp((double)logit[e] - (double)mx);
+      for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     }
+    for (int e = lane; e < E; e += 32) {
+      const double l = (double)logit[e];
+      key[e] = rank_key((r.scoring == 0 ? exp(l - (double)mx) / all : 1.0 / (1.0 + exp(-l))) + (double)r.bias[e]);
+    }
+    __syncwarp();
+    mine = pick(key, E, r.k, lane);
   }
   float s = 0.0f;
   if (lane < r.k) {
@@ -344,14 +349,17 @@ __device__ void route_token(const RouteArgs& r, const float* logit, unsigned lon
     s = r.scoring == 0 ? expf(l - mx) : 1.0f / (1.0f + expf(-l));
   }
   const float sum = warp_sum(s);
+  // a sum below the smallest normal number (every chosen score underflowed)
+  // divides as that number: weights of zero, not NaN
+  float den = r.normalize ? fmaxf(sum, 1.17549435e-38f) : 1.0f;
+  if (!r.normalize && r.scoring == 0) {
+    float all = 0.0f;
+    for (int e = lane; e < E; e += 32) all += expf(logit[e] - mx);
+    den = warp_sum(all);
+  }
   if (lane < r.k) {
-    // a sum below the smallest normal number (every chosen score underflowed)
-    // divides as that number: weights of zero, not NaN
-    const float den = r.normalize ? fmaxf(sum, 1.17549435e-38f) : r.scoring == 0 ? all : 1.0f;
-    float w = s / den * r.scale;
-    if (nan || sum != sum) w = __int_as_float(0x7FC00000);
     r.ids[(int64_t)n * slots + lane] = mine;
-    r.weights[(int64_t)n * slots + lane] = w;
+    r.weights[(int64_t)n * slots + lane] = nan || sum != sum ? __int_as_float(0x7FC00000) : s / den * r.scale;
   } else if (lane < slots) {
     r.ids[(int64_t)n * slots + lane] = E + lane - r.k;
     r.weights[(int64_t)n * slots + lane] = 1.0f;
@@ -390,12 +398,14 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
   double* part = xd + TN * CH;
   unsigned long long* key = reinterpret_cast<unsigned long long*>(part + RT_WARPS * epad * TN);
   float* logit = reinterpret_cast<float*>(key + E);
+  auto started = cl.barrier_arrive();  // this CTA runs: its shared memory may be written to
   const int tiles = (ne + RT_TE - 1) / RT_TE;
   int ks = 1;  // warps that share a tile's columns
   while (ks < RT_WARPS && ks * 2 * tiles <= RT_WARPS) ks *= 2;
   const int sl = warp % ks;
   pdl_wait();
   const bool vec = r.ldw % 4 == 0 && (reinterpret_cast<uintptr_t>(r.w) & 15) == 0;
+  const bool xvec = a.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   for (int t0 = 0; t0 < tiles; t0 += RT_WARPS / ks) {
     const int tl = t0 + warp / ks, eb = e0 + tl * RT_TE;
     double acc[RT_TE * TN] = {};
@@ -424,8 +434,8 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
         }
       }
     };
-    // the first two steps' weights are on their way while x is staged
-    constexpr int PRE = TN <= 2 ? 2 : 0;
+    // the first steps' weights are on their way while x is staged
+    constexpr int PRE = TN == 1 ? 4 : TN == 2 ? 2 : 0;
     float pre[PRE > 0 ? PRE : 1][RT_TE][4];
     if (tl < tiles)
 #pragma unroll
@@ -438,9 +448,13 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
       // reads its four columns with two conflict-free 16-byte loads
       const int cr = (cn + 127) & ~127;
       for (int n = 0; n < TN; ++n)
-        for (int c = threadIdx.x; c < cr; c += RT_THREADS) {
-          const double v = n < nn && c < cn ? load_as_f64(a.x, a.xdt, (int64_t)(n0 + n) * a.ldx + c0 + c) : 0.0;
-          xd[n * CH + (c & ~127) + ((c >> 1) & 1) * 64 + ((c >> 2) & 31) * 2 + (c & 1)] = v;
+#pragma unroll 4
+        for (int c = threadIdx.x * 4; c < cr; c += RT_THREADS * 4) {
+          float v[4];
+          load4(v, a.x, a.xdt, (int64_t)(n0 + min(n, nn - 1)) * a.ldx + c0 + c, n < nn ? cn - c : 0, xvec);
+          double* d = xd + n * CH + (c & ~127) + ((c >> 2) & 31) * 2;
+          *reinterpret_cast<double2*>(d) = make_double2((double)v[0], (double)v[1]);
+          *reinterpret_cast<double2*>(d + 64) = make_double2((double)v[2], (double)v[3]);
         }
       __syncthreads();
       if (tl < tiles) {
@@ -477,7 +491,8 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
       if ((lane & (32 / V - 1)) == 0 && e < ne) part[(sl * epad + e) * TN + at % TN] = acc[0];
     }
   }
-  cl.sync();  // every CTA of the cluster runs, and every partial sum is there
+  __syncthreads();  // every partial sum is there
+  cl.barrier_wait(std::move(started));
   for (int i = threadIdx.x; i < ne * nn; i += RT_THREADS) {
     const int e = i / nn, n = i % nn;
     double v = 0.0;
@@ -490,7 +505,7 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
 }
 
 // --------------------------------------------------- entries of the experts
-// The chosen experts in ascending order, each with up to MOE_ENT of its tokens
+// The chosen experts in ascending order (one token's: in its order), each with up to MOE_ENT of its tokens
 // (an expert with more has several entries), built by every CTA for itself from
 // the choices.  A choice outside [0, E) selects nothing; an expert that one
 // token names twice counts once, with the sum of the weights.  An expert's
@@ -518,6 +533,11 @@ __host__ __device__ __forceinline__ size_t table_bytes(int E, int P, int max_ent
   return (size_t)(3 * E + max_ent + 3 * P) * 4;
 }
 
+// No expert has tokens yet: before build_table, and before the choices are known.
+__device__ __forceinline__ void clear_table(uint8_t* mem, const MoeArgs& a) {
+  for (int i = threadIdx.x; i < 2 * a.E; i += blockDim.x) reinterpret_cast<uint32_t*>(mem)[i] = 0u;
+  __syncthreads();
+}
 template <int MOE_ENT>
 __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   __shared__ uint32_t wsum[32];
@@ -529,28 +549,38 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   t.tmp = t.ent + a.max_ent;
   t.sorted = t.tmp + P;
   t.w = reinterpret_cast<float*>(t.sorted + P);
-  for (int i = tid; i < 2 * a.E; i += blockDim.x) t.mask[i] = 0u;
-  for (int i = tid; i < P; i += blockDim.x) {
-    t.sorted[i] = (uint32_t)a.ids[i];
-    t.w[i] = a.weights[i];
-  }
-  __syncthreads();
-  for (int p = tid; p < P; p += blockDim.x) {
-    const uint32_t id = t.sorted[p];
-    const int first = p / a.slots * a.slots;
-    bool keep = id < (uint32_t)a.E;
-    for (int q = first; q < p; ++q) keep &= t.sorted[q] != id;
-    uint32_t v = 0xFFFFFFFFu;
-    if (keep) {
-      float w = t.w[p];
-      for (int q = p + 1; q < first + a.slots; ++q)
-        if (t.sorted[q] == id) w += t.w[q];  // a later duplicate's own entry is not written
-      t.w[p] = w;
-      const int n = p / a.slots;
-      atomicOr(&t.mask[2 * id + (n >> 5)], 1u << (n & 31));
-      v = id;
+  if (a.N == 1) {  // a lane per choice: an entry for each distinct expert, in their order
+    if (warp == 0) {
+      const uint32_t id = lane < P ? (uint32_t)a.ids[lane] : 0xFFFFFFFFu;
+      const float w = lane < P ? a.weights[lane] : 0.0f;
+      const uint32_t same = __match_any_sync(0xffffffffu, id);
+      const bool keep = id < (uint32_t)a.E && lane == __ffs(same) - 1;
+      const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+      float sum = 0.0f;
+      for (int i = 0; i < P; ++i) {
+        const float v = __shfl_sync(0xffffffffu, w, i);
+        if ((same >> i) & 1u) sum += v;
+      }
+      if (keep) {
+        const int i = __popc(kept & ((1u << lane) - 1u));
+        t.ent[i] = id | (uint32_t)i << 10 | 1u << 22;
+        t.sorted[i] = (uint32_t)lane;
+        t.w[lane] = sum;
+        t.mask[2 * id] = 1u;  // run() counts its tokens
+      }
+      if (lane == 0) wsum[0] = (uint32_t)__popc(kept);
     }
-    t.tmp[p] = v;
+    __syncthreads();
+    t.nent = (int)wsum[0];
+    t.per_entry = MOE_ENT;
+    return t;
+  }
+  for (int p = tid; p < P; p += blockDim.x) {
+    const uint32_t id = (uint32_t)a.ids[p];
+    const int n = p / a.slots;
+    t.tmp[p] = id;
+    t.w[p] = a.weights[p];
+    if (id < (uint32_t)a.E) atomicOr(&t.mask[2 * id + (n >> 5)], 1u << (n & 31));
   }
   __syncthreads();
   // exclusive prefix sums of the counts (low half) and the entries (high half)
@@ -585,8 +615,15 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   __syncthreads();
   for (int p = tid; p < P; p += blockDim.x) {
     const uint32_t id = t.tmp[p];
-    if (id != 0xFFFFFFFFu) {
-      const int n = p / a.slots;
+    const int n = p / a.slots;
+    bool keep = id < (uint32_t)a.E;  // the token's first choice of this expert
+    for (int q = n * a.slots; q < p; ++q) keep &= t.tmp[q] != id;
+    if (keep) {
+      // its duplicates' weights are only read, their own entries not written
+      float w = t.w[p];
+      for (int q = p + 1; q < (n + 1) * a.slots; ++q)
+        if (t.tmp[q] == id) w += t.w[q];
+      t.w[p] = w;
       const uint32_t lo = t.mask[2 * id], hi = t.mask[2 * id + 1], below = (1u << (n & 31)) - 1u;
       const int rank = n < 32 ? __popc(lo & below) : __popc(lo) + __popc(hi & below);
       t.sorted[t.first[id] + rank] = (uint32_t)p | (uint32_t)n << 16;
@@ -860,10 +897,12 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
   constexpr int SG = slab_groups<FMT>(), GB = grp_bytes<FMT>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) pipe.init();
+  uint8_t* const table = up_smem + ring_bytes<FMT>() + sizeof(UpPart<DIG>);
+  clear_table(table, a);
   pdl_wait();
   pdl_trigger();
   UpPart<DIG>& part = *reinterpret_cast<UpPart<DIG>*>(up_smem + ring_bytes<FMT>());
-  const Table tb = build_table<ent_tok<DIG>()>(up_smem + ring_bytes<FMT>() + sizeof(UpPart<DIG>), a);
+  const Table tb = build_table<ent_tok<DIG>()>(table, a);
   const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F), ns = (kg + SG - 1) / SG;
   const int units = tb.nent * fc, G = gridDim.x;
   // unit u: entry u / fc, chunk u % fc, stepped without divisions
@@ -1003,7 +1042,9 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
   for (int i = threadIdx.x; i < MOE_KS * yn; i += DN_THREADS) ypart[i] = 0.0f;
   // the choices were complete before k_moe_up passed its own wait and
   // allowed this launch; what k_moe_up writes comes after the wait below
-  const Table tb = build_table<ent_tok<DIG>()>(dn_smem + ring_bytes<FMT>() + (size_t)MOE_KS * yn * 4, a);
+  uint8_t* const table = dn_smem + ring_bytes<FMT>() + (size_t)MOE_KS * yn * 4;
+  clear_table(table, a);
+  const Table tb = build_table<ent_tok<DIG>()>(table, a);
   const int fg = groups_of(a.F), fs = (fg + SG - 1) / SG, chunks = (a.K + R - 1) / R;
   const int64_t total = (int64_t)tb.nent * fs;
   const int q0 = (int)(total * rank / cs), q1 = (int)(total * (rank + 1) / cs);
@@ -1205,6 +1246,38 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
   return OK;
 }
 
+// Clusters of `cs` CTAs of a kernel that are resident at once (cached; kernels
+// that leave one CTA per SM whatever the call's shared memory).
+int active_clusters(const void* f, const DeviceInfo& dev, int threads, size_t smem, int cs, int* out) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int>, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_tuple(f, dev.device, cs);
+  const auto it = known.find(key);
+  if (it != known.end()) {
+    *out = it->second;
+    return OK;
+  }
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cs);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, f, &cfg);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(ERR_CUDA, "resident clusters of %d: %s", cs, cudaGetErrorString(e));
+  }
+  *out = known[key] = n;
+  return OK;
+}
+
 // Clusters of more than 8 CTAs are opt-in per kernel (and device).
 int allow_cluster16(const void* f, const DeviceInfo& dev) {
   static std::mutex mu;
@@ -1276,8 +1349,16 @@ int launch_down(const MoeArgs& a, int ydt, const DeviceInfo& dev, cudaStream_t s
   if (int rc = allow_max_smem((const void*)k_moe_down<FMT, DIG>, dev)) return rc;
   const size_t smem = dn_smem<FMT>(a.E, a.N * a.slots, a.max_ent, a.N);
   const int chunks = (a.K + 16 * MOE_RT - 1) / (16 * MOE_RT);
-  // CTAs that share 64 rows: as many as the device holds at once, one per SM
-  const int cs = std::max(1, std::min(MOE_DOWN_CL, dev.sms / chunks));
+  // CTAs that share 64 rows: as many as leaves every cluster resident at once
+  // (one CTA per SM; a GPC's SMs do not divide by every size: 23 clusters of 6
+  // took two turns)
+  int cs = MOE_DOWN_CL;
+  while (cs > 1) {
+    int most = 0;
+    if (int rc = active_clusters((const void*)k_moe_down<FMT, DIG>, dev, DN_THREADS, smem, cs, &most)) return rc;
+    if (chunks <= most) break;
+    --cs;
+  }
   return launch("k_moe_down", k_moe_down<FMT, DIG>, dim3(chunks * cs), DN_THREADS, smem, cs, st, a, ydt);
 }
 
