@@ -784,13 +784,13 @@ struct Digits {
   uint4 b[2];
   uint4 s;
 };
-template <int DIG>
+// Where a lane finds the digits and scales of one MMA's tokens: group 0's.
 struct Cols {
   const uint8_t* dig;
   const float* s;
   // row(i): the activation row of the i-th of `cnt` tokens; the columns of
   // absent tokens repeat the last one's
-  template <typename Row>
+  template <int DIG, typename Row>
   __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups, int cnt,
                                       int lane, Row row) {
     const int n = lane >> 2, t = lane & 3;
@@ -800,11 +800,16 @@ struct Cols {
     dig = digits + row(min(tok, cnt - 1)) * groups * dig_bytes<DIG>() + d * 128 + t * 32;
     s = scales + row(min(DIG == 2 ? t : t >> 1, cnt - 1)) * groups * 4;
   }
-  __device__ __forceinline__ void load(Digits& f, int grp) const {
-    const uint8_t* p = dig + grp * dig_bytes<DIG>();
-    f.b[0] = ldg128(p);
-    f.b[1] = ldg128(p + 16);
-    f.s = ldg128(s + grp * 4);
+  // group j from here
+  template <int DIG>
+  __device__ __forceinline__ void load(Digits& f, int j) const {
+    f.b[0] = ldg128(dig + j * dig_bytes<DIG>());
+    f.b[1] = ldg128(dig + j * dig_bytes<DIG>() + 16);
+    f.s = ldg128(s + j * 4);
+  }
+  template <int DIG>
+  __device__ __forceinline__ Cols at(int grp) const {
+    return Cols{dig + (int64_t)grp * dig_bytes<DIG>(), s + (int64_t)grp * 4};
   }
 };
 
@@ -823,47 +828,99 @@ __device__ __forceinline__ void product(float* acc, const Quants<FMT>& q, const 
   }
 }
 
-// What a compute warp holds: its entry's tokens (one or two MMAs of them),
-// their digits of two groups in turn, and its 16 rows' sums.
+// What a compute warp holds: the digits of the slab at hand, read a slab ahead
+// (they come from L2: a group ahead left the warps waiting), and its 16 rows'
+// sums.  Four sets of digits fit the registers: two groups of one or two MMAs
+// of tokens (q8_0), four groups of one MMA (q4_0); a q4_0 slab with two MMAs
+// keeps two groups and reads on inside the slab.
 template <int FMT, int DIG>
 struct Work {
   static constexpr int T = tok_mma<DIG>(), SG = slab_groups<FMT>();
-  Cols<DIG> c0, c1;
-  Digits f[2][2];  // [even, odd group][MMA]
+  // the slab ahead: its tokens' digits (of its first group), groups and width
+  struct Ahead {
+    Cols c0, c1;
+    int m = 0;  // 0: none
+    bool two = false;
+  };
+  Cols e0, e1;  // the entry ahead, from its first group
+  bool etwo;
+  Digits f[4];
   float acc[4];
-  bool two;
-  // the entry's tokens; row(i) as in Cols
+  // the next slabs' entry: its tokens; row(i) as in Cols
   template <typename Row>
   __device__ __forceinline__ void entry(const uint8_t* digits, const float* scales, int groups, int cnt,
                                         int lane, Row row) {
-    two = cnt > T;
-    c0.set(digits, scales, groups, cnt, lane, row);
-    if (two) c1.set(digits, scales, groups, cnt - T, lane, [&](int i) { return row(T + i); });
+    etwo = cnt > T;
+    e0.template set<DIG>(digits, scales, groups, cnt, lane, row);
+    if (etwo) e1.template set<DIG>(digits, scales, groups, cnt - T, lane, [&](int i) { return row(T + i); });
   }
-  __device__ __forceinline__ void load(int buf, int grp) {
-    c0.load(f[buf][0], grp);
-    if (two) c1.load(f[buf][1], grp);
+  __device__ __forceinline__ Ahead ahead(int grp, int m) const {
+    Ahead a;
+    a.c0 = e0.template at<DIG>(grp);
+    a.c1 = e1.template at<DIG>(grp);
+    a.m = m;
+    a.two = etwo;
+    return a;
+  }
+  __host__ __device__ static constexpr bool whole(bool two) { return SG == 2 || !two; }  // all of a slab's digits fit
+  __host__ __device__ static constexpr int slot(bool two, int j, int c) {
+    return SG == 2 ? j * 2 + c : two ? (j & 1) * 2 + c : j;
+  }
+  template <bool TWO>
+  __device__ __forceinline__ void load(const Ahead& a, int j) {
+    a.c0.template load<DIG>(f[slot(TWO, j, 0)], j);
+    if (TWO) a.c1.template load<DIG>(f[slot(TWO, j, 1)], j);
+  }
+  // what a slab starts with
+  __device__ __forceinline__ void begin(const Ahead& a) {
+#pragma unroll
+    for (int j = 0; j < SG; ++j) {
+      if (j >= a.m) break;
+      if (a.two) {
+        if (whole(true) || j < 2) load<true>(a, j);
+      } else {
+        load<false>(a, j);
+      }
+    }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
   }
-  // m groups from grp on; the first one's digits are in f[0]
-  __device__ __forceinline__ void slab(uint32_t st, int rt, int grp, int m, int lane) {
+  template <bool TWO>
+  __device__ __forceinline__ void groups(uint32_t st, const Ahead& now, const Ahead& next, int lane) {
     const int w = DIG == 3 && (lane & 1) ? 0 : 256;
-    st += rt * grp_bytes<FMT>();
+    const int nm = whole(TWO) && next.two == TWO ? next.m : 0;
 #pragma unroll
     for (int j = 0; j < SG; ++j) {
-      if (j > 0 && j >= m) break;
-      if (j + 1 < m) load((j + 1) & 1, grp + j + 1);
+      if (j > 0 && j >= now.m) break;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         Quants<FMT> q;
         q.load(st + j * MOE_RT * grp_bytes<FMT>(), p, lane);
-        product<FMT>(acc, q, f[j & 1][0], p, w);
-        if (two) product<FMT>(acc + 2, q, f[j & 1][1], p, w);
+        product<FMT>(acc, q, f[slot(TWO, j, 0)], p, w);
+        if (TWO) product<FMT>(acc + 2, q, f[slot(TWO, j, 1)], p, w);
+      }
+      if (whole(TWO)) {
+        if (j < nm) load<TWO>(next, j);
+      } else if (j + 2 < now.m) {
+        load<TWO>(now, j + 2);
       }
     }
+    // groups of a longer next slab that this one had none for, or all of them
+    if (nm > 0) {
+#pragma unroll
+      for (int j = 1; j < SG; ++j)
+        if (j >= now.m && j < nm) load<TWO>(next, j);
+    } else {
+      begin(next);
+    }
+  }
+  // the slab `now`, whose digits are there or on their way; asks for `next`'s
+  __device__ __forceinline__ void slab(uint32_t st, int rt, const Ahead& now, const Ahead& next, int lane) {
+    st += rt * grp_bytes<FMT>();
+    if (now.two) groups<true>(st, now, next, lane);
+    else groups<false>(st, now, next, lane);
   }
   // put(token of the entry, row g's sum, row g + 8's sum) for every token that
   // this lane holds
@@ -949,38 +1006,62 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
     const int rt = warp % MOE_RT, kq = warp / MOE_RT;
     Work<FMT, DIG> w;
     w.clear();
-    // unit number here, slab, the unit's first slab of this split (slab i of the
-    // CTA is split i % 3's, counted on through the units)
-    int j = 0, l = kq, l0 = kq, chunk;
+    // the unit whose sums are under way (number j here, entry en) and the slab
+    // ahead: slab i of the CTA is split i % 3's, counted on through the units
     const int shift = ns % MOE_KS;
+    auto first_slab = [&](int l0) { return l0 >= shift ? l0 - shift : l0 - shift + MOE_KS; };
+    int j = 0, l = kq, l0 = kq, al = kq, al0 = kq, chunk;
     Turn turn{kq};
-    uint32_t en = 0;
+    Pos here = pos;  // `pos` runs ahead
     auto take = [&]() {
-      en = unit(chunk);
+      const uint32_t en = unit(chunk);
       const int at = (en >> 10) & 0xFFF;
-      w.entry(a.xdig, a.xs, kg, (en >> 22) & 15, lane,
-              [&](int i) { return (int64_t)(tb.sorted[at + i] >> 16); });
-      if (l < ns) w.load(0, l * SG);
+      w.entry(a.xdig, a.xs, kg, (en >> 22) & 15, lane, [&](int i) { return (int64_t)(tb.sorted[at + i] >> 16); });
     };
-    bool more = pos.u < units;
-    if (more) take();
-    while (more) {
+    auto peek = [&]() {  // the slab ahead, over units that have none for this split
+      typename Work<FMT, DIG>::Ahead x;
+      bool moved = false;
+      while (al >= ns) {
+        step();
+        if (pos.u >= units) return x;
+        al0 = first_slab(al0);
+        al = al0;
+        moved = true;
+      }
+      if (moved) take();
+      return w.ahead(al * SG, min(SG, kg - al * SG));
+    };
+    typename Work<FMT, DIG>::Ahead now;
+    if (pos.u < units) {
+      take();
+      now = peek();
+      w.begin(now);
+    }
+    while (here.u < units) {
       while (l < ns) {
+        al += MOE_KS;
+        const auto next = peek();
         if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
-        w.slab(saddr(up_smem) + turn.s * slab_bytes<FMT>(), rt, l * SG, min(SG, kg - l * SG), lane);
+        w.slab(saddr(up_smem) + turn.s * slab_bytes<FMT>(), rt, now, next, lane);
         __syncwarp();  // every lane has read the stage
         if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
         turn.next();
+        now = next;
         l += MOE_KS;
-        if (l < ns) w.load(0, l * SG);
       }
       if (l < ns) break;  // gave up
-      // this unit's sums; the next unit's first digits are on their way meanwhile
-      const int cnt = (en >> 22) & 15, b = j & 1;
-      l0 = l0 >= shift ? l0 - shift : l0 - shift + MOE_KS;
+      // this unit's sums
+      const int b = j & 1;
+      const Pos ran = pos;
+      pos = here;
+      const uint32_t en = unit(chunk);
+      step();
+      here = pos;
+      pos = ran;
+      l0 = first_slab(l0);
       l = l0;
       if (j >= 2 && !mbar_wait(saddr(&pipe.pempty[b]), (uint32_t)(j / 2 - 1) & 1u, &pipe.abort_flag)) break;
-      w.each(cnt, lane, [&](int i, float gate, float up) {
+      w.each((en >> 22) & 15, lane, [&](int i, float gate, float up) {
         float* p = part.v[b][kq][i] + rt * 8 + (lane >> 2);
         p[0] = gate;
         p[32] = up;
@@ -989,9 +1070,6 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(saddr(&pipe.pfull[b]));
       ++j;
-      step();
-      more = pos.u < units;
-      if (more) take();
     }
   } else {
     // -------------------------------------------------------------- finish
@@ -1071,50 +1149,55 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
     float* yp = ypart + kq * yn + rt * 16 + (lane >> 2);
     Work<FMT, DIG> w;
     w.clear();
-    int q = q0 + kq, e = q / fs, l = q - e * fs;
+    // slab q of entry e (`en`: its tokens), and the slab ahead (al of entry ae)
+    int q = q0 + kq, ae = q / fs, al = q - ae * fs;
     Turn turn{kq};
-    uint32_t en = 0;
-    auto take = [&]() {
-      en = tb.ent[e];
+    auto take = [&](uint32_t en) {
       const int at = (en >> 10) & 0xFFF;
-      w.entry(a.hdig, a.hs, fg, (en >> 22) & 15, lane,
-              [&](int i) { return (int64_t)(tb.sorted[at + i] & 0xFFFFu); });
+      w.entry(a.hdig, a.hs, fg, (en >> 22) & 15, lane, [&](int i) { return (int64_t)(tb.sorted[at + i] & 0xFFFFu); });
     };
+    typename Work<FMT, DIG>::Ahead now;
+    uint32_t en = 0;
     if (q < q1) {
-      take();
-      w.load(0, l * SG);
+      en = tb.ent[ae];
+      take(en);
+      now = w.ahead(al * SG, min(SG, fg - al * SG));
+      w.begin(now);
     }
     while (q < q1) {
+      typename Work<FMT, DIG>::Ahead next;
+      uint32_t nen = en;
+      q += MOE_KS;
+      if (q < q1) {
+        al += MOE_KS;
+        if (al >= fs) {
+          do {
+            al -= fs;
+            ++ae;
+          } while (al >= fs);
+          nen = tb.ent[ae];
+          take(nen);
+        }
+        next = w.ahead(al * SG, min(SG, fg - al * SG));
+      }
       if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
-      w.slab(saddr(dn_smem) + turn.s * slab_bytes<FMT>(), rt, l * SG, min(SG, fg - l * SG), lane);
+      w.slab(saddr(dn_smem) + turn.s * slab_bytes<FMT>(), rt, now, next, lane);
       __syncwarp();  // every lane has read the stage
       if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
       turn.next();
-      q += MOE_KS;
-      l += MOE_KS;
-      if (l < fs && q < q1) {
-        w.load(0, l * SG);
-        continue;
+      now = next;
+      if (nen != en || q >= q1) {  // that was the entry's last slab of this warp
+        const int at = (en >> 10) & 0xFFF;
+        // tokens of an entry are distinct, and the rows are this warp's own
+        w.each((en >> 22) & 15, lane, [&](int k, float lo, float hi) {
+          float* p = yp + (tb.sorted[at + k] >> 16) * R;
+          p[0] += lo;
+          p[8] += hi;
+        });
+        w.clear();
+        __syncwarp();  // the next entry may add to the same token from other lanes
+        en = nen;
       }
-      // the entry's last slab of this warp: its sums, the next entry's first
-      // digits on their way meanwhile
-      const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15;
-      if (q < q1) {
-        while (l >= fs) {
-          l -= fs;
-          ++e;
-        }
-        take();
-        w.load(0, l * SG);
-      }
-      // tokens of an entry are distinct, and the rows are this warp's own
-      w.each(cnt, lane, [&](int k, float lo, float hi) {
-        float* p = yp + (tb.sorted[at + k] >> 16) * R;
-        p[0] += lo;
-        p[8] += hi;
-      });
-      w.clear();
-      __syncwarp();  // the next entry may add to the same token from other lanes
     }
   }
   cl.sync();
