@@ -240,7 +240,7 @@ constexpr int RT_WARPS = RT_THREADS / 32;
 template <int TN> __host__ __device__ constexpr int rt_cl() { return TN == 1 ? 16 : 8; }
 constexpr int RT_TE = 4;    // experts of a warp's tile
 // x columns staged at a time, as doubles (32 KB)
-template <int TN> __host__ __device__ constexpr int rt_chunk() { return TN == 1 ? 4096 : TN == 2 ? 2048 : 512; }
+template <int TN> __host__ __device__ constexpr int rt_chunk() { return TN == 1 ? 4096 : 2048; }
 
 // Ordering keys of a score: larger key = larger score, +0 == -0, NaN lowest (1;
 // 0 marks a taken expert).
@@ -435,8 +435,8 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
       }
     };
     // the first steps' weights are on their way while x is staged
-    constexpr int PRE = TN == 1 ? 4 : TN == 2 ? 2 : 0;
-    float pre[PRE > 0 ? PRE : 1][RT_TE][4];
+    constexpr int PRE = TN == 1 ? 4 : 2;
+    float pre[PRE][RT_TE][4];
     if (tl < tiles)
 #pragma unroll
       for (int j = 0; j < PRE; ++j)
@@ -502,6 +502,94 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
   }
   cl.sync();
   if (warp == 0 && rank < nn) route_token(r, logit, key, n0 + rank, lane);
+}
+
+// Many tokens: clusters of 8 CTAs take 16 tokens; a warp 16 experts x 16 tokens
+// of a slice of the columns, on the fp64 matrix instruction m8n8k4 (the same 64
+// multiply-adds per clock and SM as DFMA, but two operand registers for 256 of
+// them): lane (r, t) reads four consecutive columns 4t ... of rows r and r + 8 of
+// both matrices straight into fragments, so nothing is staged.
+constexpr int RM_TN = 16, RM_CL = 8, RM_TE = 16;
+__device__ __forceinline__ void dmma(double (&c)[2], double a, double b) {
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+      : "+d"(c[0]), "+d"(c[1])
+      : "d"(a), "d"(b));
+}
+__host__ __device__ constexpr int rm_slices(int ne) {  // warps that share a tile's columns
+  int ks = 1;
+  while (ks < RT_WARPS && ks * 2 * ((ne + RM_TE - 1) / RM_TE) <= RT_WARPS) ks *= 2;
+  return ks;
+}
+__global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route_many(MoeArgs a, RouteArgs r) {
+  extern __shared__ __align__(16) uint8_t rt_smem[];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int)blockIdx.x >= RM_CL * r.clusters) {
+    pdl_wait();
+    const int w = (blockIdx.x - RM_CL * r.clusters) * RT_WARPS + warp;
+    const int nw = (gridDim.x - RM_CL * r.clusters) * RT_WARPS;
+    if (a.xdt == 0) prepare_x<3>(a, w, nw, lane);
+    else prepare_x<2>(a, w, nw, lane);
+    return;
+  }
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), E = r.E, K = r.K;
+  const int n0 = (blockIdx.x / RM_CL) * RM_TN, nn = min(RM_TN, a.N - n0);
+  const int e0 = (int)((int64_t)E * rank / RM_CL), e1 = (int)((int64_t)E * (rank + 1) / RM_CL);
+  const int ne = e1 - e0, epad = (E + RM_CL - 1) / RM_CL;
+  // shared memory: keys of two tokens [2][E], partial sums [slices][epad][16],
+  // the logits of this CTA's tokens (rank and rank + 8) [2][E]
+  const int kmax = rm_slices(epad);  // the same layout in every CTA of the cluster
+  unsigned long long* key = reinterpret_cast<unsigned long long*>(rt_smem);
+  double* part = reinterpret_cast<double*>(key + 2 * E);
+  float* logit = reinterpret_cast<float*>(part + kmax * epad * RM_TN);
+  auto started = cl.barrier_arrive();  // this CTA runs: its shared memory may be written to
+  const int tiles = (ne + RM_TE - 1) / RM_TE, ks = kmax, sl = warp % ks;
+  const int row = lane >> 2, t = lane & 3;
+  const bool vec = r.ldw % 4 == 0 && (reinterpret_cast<uintptr_t>(r.w) & 15) == 0;
+  const bool xvec = a.ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  pdl_wait();
+  for (int tl = warp / ks; tl < tiles; tl += RT_WARPS / ks) {
+    const int eb = e0 + tl * RM_TE;
+    double acc[2][2][2] = {};
+    const int64_t w0 = (int64_t)min(eb + row, e1 - 1) * r.ldw, w1 = (int64_t)min(eb + 8 + row, e1 - 1) * r.ldw;
+    const int64_t x0 = (int64_t)(n0 + min(row, nn - 1)) * a.ldx, x1 = (int64_t)(n0 + min(8 + row, nn - 1)) * a.ldx;
+#pragma unroll 2
+    for (int cb = sl * 16; cb < K; cb += ks * 16) {  // every lane takes part to the end
+      const int c = cb + 4 * t;
+      float fw[2][4], fx[2][4];
+      load4(fw[0], r.w, r.wdt, w0 + c, K - c, vec);
+      load4(fw[1], r.w, r.wdt, w1 + c, K - c, vec);
+      load4(fx[0], a.x, a.xdt, x0 + c, K - c, xvec);
+      load4(fx[1], a.x, a.xdt, x1 + c, K - c, xvec);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) dmma(acc[p][q], (double)fw[p][i], (double)fx[q][i]);
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int e = eb + 8 * p + row - e0, n = 8 * q + 2 * t + i;
+          if (e < ne) part[(sl * epad + e) * RM_TN + n] = acc[p][q][i];
+        }
+  }
+  __syncthreads();  // every partial sum is there
+  cl.barrier_wait(std::move(started));
+  for (int i = threadIdx.x; i < ne * nn; i += RT_THREADS) {
+    const int e = i / nn, n = i % nn;
+    double v = 0.0;
+    for (int s = 0; s < ks; ++s) v += part[(s * epad + e) * RM_TN + n];
+    cl.map_shared_rank(logit, n % RM_CL)[(n / RM_CL) * E + e0 + e] = (float)v;
+  }
+  cl.sync();
+  if (warp < RM_TN / RM_CL && rank + RM_CL * warp < nn)
+    route_token(r, logit + warp * E, key + warp * E, n0 + rank + RM_CL * warp, lane);
 }
 
 // --------------------------------------------------- entries of the experts
@@ -1403,10 +1491,17 @@ int launch_route_n(const MoeArgs& a, RouteArgs& r, bool route, bool prep, const 
 int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const DeviceInfo& dev,
                  cudaStream_t st) {
   // up to 32 tokens two to a cluster (latency counts: the clusters run side by
-  // side), above that eight (the router's weights are read an eighth as often)
+  // side), above that sixteen on matrix instructions (512 tokens, 256 experts of
+  // 4096 columns: 8 tokens a cluster on DFMA 230 us, @@512)
   if (a.N == 1) return launch_route_n<1>(a, r, route, prep, dev, st);
   if (a.N <= 32) return launch_route_n<2>(a, r, route, prep, dev, st);
-  return launch_route_n<8>(a, r, route, prep, dev, st);
+  r.clusters = route ? (a.N + RM_TN - 1) / RM_TN : 0;
+  int pre = prep ? (int)std::min<int64_t>(((int64_t)a.N * groups_of(a.K) + RT_WARPS - 1) / RT_WARPS, 2 * dev.sms) : 0;
+  pre = (pre + RM_CL - 1) / RM_CL * RM_CL;
+  if (int rc = allow_max_smem((const void*)k_moe_route_many, dev)) return rc;
+  const int epad = (r.E + RM_CL - 1) / RM_CL;
+  const size_t smem = route ? (size_t)r.E * 24 + (size_t)rm_slices(epad) * epad * RM_TN * 8 : 0;
+  return launch("k_moe_route", k_moe_route_many, dim3(RM_CL * r.clusters + pre), RT_THREADS, smem, RM_CL, st, a, r);
 }
 
 template <int FMT, int DIG>
