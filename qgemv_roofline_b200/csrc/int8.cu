@@ -15,12 +15,12 @@
 // past the end read as zeros.  TMEM lane = channel, column = token: a warp
 // stores 32 consecutive channels of a token at a time.  Two kernels:
 //
-//  * k_int8_mm (few tiles): one tile of 128 channels x 16 to 128 tokens per CTA
+//  * k_int8_mm (up to 128 tokens): one tile of 128 channels x 16 to 128 tokens per CTA
 //    or, where there are fewer tiles than CTAs, per cluster, whose CTAs split K
 //    and add their int32 parts through distributed shared memory (exact in any
 //    order).  With one token the weights' stream is what counts.
-//  * k_int8_pair (many): persistent CTA pairs (tcgen05 cta_group::2) on tiles of
-//    256 channels x 256 tokens; each CTA copies its half of both operands, so
+//  * k_int8_pair (more): persistent CTA pairs (tcgen05 cta_group::2) on tiles of
+//    256 channels x up to 256 tokens; each CTA copies its half of both operands, so
 //    that an SM reads 64 instead of 96 bytes of shared memory per cycle; two
 //    accumulators in TMEM, so that one tile is stored while the next is summed.
 #include <algorithm>
@@ -90,12 +90,12 @@ __device__ __forceinline__ int quant1(float v, float s, float inv, bool exact) {
 }
 
 constexpr int RQ_THREADS = 256;
-constexpr int RQ_HELD = 4;  // vectors of 8 values that a thread keeps
+constexpr int RQ_HELD = 2;  // vectors of 8 values that a thread keeps
 
 // One CTA per row.  A row with a NaN or an infinity gets the scale NaN and
 // zeros; an all-zero row (or one whose scale underflows to 0) the scale 0 and
 // zeros.  VEC: rows start on 16-byte boundaries, q's on 8-byte ones, and K is a
-// multiple of 8: a row of up to 8192 values is read once and kept.
+// multiple of 8: a row of up to 4096 values is read once and kept.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__ x, int64_t ldx, int K,
                                                            int8_t* __restrict__ q, int64_t ldq,
@@ -106,36 +106,34 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
   int8_t* qr = q + row * ldq;
-  auto load8 = [&](float (&v)[8], int i) {  // values 8 i ...
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(xr)[2 * i], b = reinterpret_cast<const float4*>(xr)[2 * i + 1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 a = reinterpret_cast<const uint4*>(xr)[i];
-      const T* t = reinterpret_cast<const T*>(&a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = as_f32(t[j]);
-    }
+  // 8 values as they are read (kept so, for registers: the kernel is many short
+  // CTAs, and 64 registers a thread halved how many an SM holds)
+  struct Raw {
+    uint4 u[sizeof(T) / 2];
   };
+  auto load8 = [&](Raw& r, int i) {  // values 8 i ...
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) r.u[j] = reinterpret_cast<const uint4*>(xr)[i * (int)(sizeof(T) / 2) + j];
+  };
+  auto value = [](const Raw& r, int j) { return as_f32(reinterpret_cast<const T*>(&r)[j]); };
   auto bits = [](float v) { return __float_as_uint(v) & 0x7FFFFFFFu; };
   uint32_t m = 0u;
-  float held[RQ_HELD][8];
+  Raw held[RQ_HELD];
   const int nv = K / 8;
   if (VEC) {
 #pragma unroll
-    for (int h = 0; h < RQ_HELD; ++h) {
-      const int i = threadIdx.x + h * RQ_THREADS;
-      if (i < nv) {
-        load8(held[h], i);
+    for (int h = 0; h < RQ_HELD; ++h)
+      if (threadIdx.x + h * RQ_THREADS < nv) load8(held[h], threadIdx.x + h * RQ_THREADS);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, bits(held[h][j]));
-      }
-    }
+    for (int h = 0; h < RQ_HELD; ++h)
+      if (threadIdx.x + h * RQ_THREADS < nv)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, bits(value(held[h], j)));
     for (int i = threadIdx.x + RQ_HELD * RQ_THREADS; i < nv; i += RQ_THREADS) {
-      float v[8];
+      Raw v;
       load8(v, i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, bits(v[j]));
+      for (int j = 0; j < 8; ++j) m = max(m, bits(value(v, j)));
     }
   } else {
     for (int k = threadIdx.x; k < K; k += RQ_THREADS) m = max(m, bits(as_f32(xr[k])));
@@ -151,11 +149,11 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
   const float inv = some ? __fdiv_rn(1.0f, sc) : 0.0f;
   if (threadIdx.x == 0) s[row] = sc;
   if (VEC) {
-    auto put8 = [&](const float (&v)[8], int i) {
+    auto put8 = [&](const Raw& v, int i) {
       uint32_t w[2] = {0u, 0u};
       if (some) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(quant1(v[j], sc, inv, exact) & 0xFF) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(quant1(value(v, j), sc, inv, exact) & 0xFF) << (8 * (j & 3));
       }
       reinterpret_cast<uint2*>(qr)[i] = make_uint2(w[0], w[1]);
     };
@@ -165,7 +163,7 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
       if (i < nv) put8(held[h], i);
     }
     for (int i = threadIdx.x + RQ_HELD * RQ_THREADS; i < nv; i += RQ_THREADS) {
-      float v[8];
+      Raw v;
       load8(v, i);
       put8(v, i);
     }
@@ -298,16 +296,21 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = tmem_base;
 
+  // the producer and the MMA warp run their loops as a whole, one elected lane
+  // issues: addresses and descriptors are then in uniform registers
   if (warp == 0) {
-    if (lane == 0) {
+    {
       const int pre = min(S, steps);
       auto load_w = [&](int i) {
-        mbar_expect_tx(saddr(&full[i % S]), C::STAGE);
-        tensor_g2s(ring_s + (i % S) * C::STAGE, &p.wmap, (k0 + i) * I8_KB, m0, saddr(&full[i % S]));
+        if (elect_one()) {
+          mbar_expect_tx(saddr(&full[i % S]), C::STAGE);
+          tensor_g2s(ring_s + (i % S) * C::STAGE, &p.wmap, (k0 + i) * I8_KB, m0, saddr(&full[i % S]));
+        }
       };
       auto load_x = [&](int i) {
-        tensor_g2s(ring_s + (i % S) * C::STAGE + I8_ABYTES, &p.xmap, (k0 + i) * I8_KB, n0,
-                   saddr(&full[i % S]));
+        if (elect_one())
+          tensor_g2s(ring_s + (i % S) * C::STAGE + I8_ABYTES, &p.xmap, (k0 + i) * I8_KB, n0,
+                     saddr(&full[i % S]));
       };
       if (p.early_w)
         for (int i = 0; i < pre; ++i) load_w(i);
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
       for (int i = 0; i < pre; ++i) load_x(i);
       int issued = pre;
       for (int i = pre; i < steps; ++i) {
-        if (!mbar_wait(saddr(&empty[i % S]), (uint32_t)((i / S - 1) & 1), &abort_flag)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(saddr(&empty[i % S]), (uint32_t)((i / S - 1) & 1), &abort_flag))) break;
         load_w(i);
         load_x(i);
         issued = i + 1;
@@ -327,24 +330,25 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
         mbar_wait_drain(saddr(&full[i % S]), (uint32_t)((i / S) & 1));
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      pdl_wait();  // so that the bounded waits below do not count the previous kernel's time
-      bool ok = true;
-      for (int i = 0; i < steps && ok; ++i) {
-        const int s = i % S;
-        ok = mbar_wait(saddr(&full[s]), (uint32_t)((i / S) & 1), &abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t da = sw128_desc(ring_s + s * C::STAGE),
-                       db = sw128_desc(ring_s + s * C::STAGE + I8_ABYTES);
+    pdl_wait();  // so that the bounded waits below do not count the previous kernel's time
+    bool ok = true;
+    for (int i = 0; i < steps && ok; ++i) {
+      const int s = i % S;
+      ok = __all_sync(0xffffffffu, mbar_wait(saddr(&full[s]), (uint32_t)((i / S) & 1), &abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t da = sw128_desc(ring_s + s * C::STAGE), db = sw128_desc(ring_s + s * C::STAGE + I8_ABYTES);
 #pragma unroll
         for (int k = 0; k < I8_KB / 32; ++k)
           tc_mma_i8<1>(tmem, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), C::IDESC, i > 0 || k > 0);
         tc_commit(saddr(&empty[s]));
       }
-      tc_commit(saddr(&done));
-      mbar_wait_drain(saddr(&done), 0u);  // no MMA outlives its operands or the accumulators
+      __syncwarp();
     }
+    if (elect_one()) tc_commit(saddr(&done));
+    __syncwarp();
+    mbar_wait_drain(saddr(&done), 0u);  // no MMA outlives its operands or the accumulators
   } else {
     pdl_wait();  // xs
     if (warp == 2) pdl_trigger();
@@ -398,23 +402,22 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
 }
 
 // ----------------------------------------------------------- CTA pairs
-constexpr int PR_N = 256;                             // tokens per tile
-constexpr int PR_STAGE = I8_ABYTES + (PR_N / 2) * I8_KB;  // a CTA's half: 32 KB
+constexpr int PR_N = 256;                             // tokens per tile, at most
+constexpr int PR_STAGE = I8_ABYTES + (PR_N / 2) * I8_KB;  // a CTA's half: up to 32 KB
 constexpr int PR_S = 6;
 constexpr int PR_EW = 8;                              // epilogue warps
 constexpr int PR_THREADS = 32 * (2 + PR_EW);
 constexpr size_t PR_SMEM = (size_t)PR_S * PR_STAGE + 1024;
-constexpr uint32_t PR_IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PR_N >> 3) << 17) |
-                              ((uint32_t)(2 * I8_M >> 4) << 24);
 
 // Tiles t = cluster, cluster + clusters, ... of (channel tile t / token tiles,
 // token tile t % token tiles): tiles under way at the same time share channel
 // tiles, and all token tiles stay in L2.  CTA 0 of the pair issues the MMAs; the
 // copies of both CTAs complete on CTA 0's `full` barriers, and its commits
-// arrive on both CTAs' `empty` and `tfull` barriers.
+// arrive on both CTAs' `empty` and `tfull` barriers.  `width` tokens per tile
+// (a multiple of 32): what fills the pairs best.
 template <typename Y>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
-    k_int8_pair(const __grid_constant__ I8Args p, int ntn, int tiles) {
+    k_int8_pair(const __grid_constant__ I8Args p, int width, int ntn, int tiles) {
   extern __shared__ uint8_t pr_smem_raw[];
   __shared__ __align__(8) unsigned long long full[PR_S], empty[PR_S], tfull[2], tempty[2];
   __shared__ uint32_t tmem_base;
@@ -426,7 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       (reinterpret_cast<uintptr_t>(pr_smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t ring_s = saddr(ring);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2, hw = width / 2;
   const int mine = pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0;  // tiles of this pair
   if (threadIdx.x == 0) {
     for (int s = 0; s < PR_S; ++s) {
@@ -455,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    {
       // a step at a time: K step k of tile t into stage s (counted, not divided:
       // one thread does all this, in the time of four MMAs)
       struct At {
@@ -470,14 +473,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
         }
       };
       auto load_w = [&](const At& at, int m0) {
-        if (rank == 0) mbar_expect_tx(saddr(&full[at.s]), 2 * PR_STAGE);
-        tensor_g2s_pair(ring_s + at.s * PR_STAGE, &p.wmap, at.k * I8_KB, m0, fbar + 8 * at.s);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(saddr(&full[at.s]), 2 * (uint32_t)(I8_ABYTES + hw * I8_KB));
+          tensor_g2s_pair(ring_s + at.s * PR_STAGE, &p.wmap, at.k * I8_KB, m0, fbar + 8 * at.s);
+        }
       };
       auto load_x = [&](const At& at, int n0) {
-        tensor_g2s_pair(ring_s + at.s * PR_STAGE + I8_ABYTES, &p.xmap, at.k * I8_KB, n0, fbar + 8 * at.s);
+        if (elect_one())
+          tensor_g2s_pair(ring_s + at.s * PR_STAGE + I8_ABYTES, &p.xmap, at.k * I8_KB, n0, fbar + 8 * at.s);
       };
       auto m_of = [&](int t) { return (t / ntn) * 2 * I8_M + (int)rank * I8_M; };
-      auto n_of = [&](int t) { return (t % ntn) * PR_N + (int)rank * (PR_N / 2); };
+      auto n_of = [&](int t) { return (t % ntn) * width + (int)rank * hw; };
       const int64_t total = (int64_t)mine * p.nk;
       const int pre = (int)min((int64_t)PR_S, total);
       At at{0, 0, pair};
@@ -493,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       uint32_t phase = 0u;
       int m0 = m_of(at.t), n0 = n_of(at.t);
       while (issued < total) {
-        if (!mbar_wait(saddr(&empty[at.s]), phase, &abort_flag)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(saddr(&empty[at.s]), phase, &abort_flag))) break;
         if (at.k == 0) {
           m0 = m_of(at.t);
           n0 = n_of(at.t);
@@ -512,36 +518,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
-    if (lane == 0 && rank == 0) {
+    // the whole warp runs the loop, one elected lane issues: what an MMA takes is
+    // then in uniform registers (a lane's own branch cost more cycles per MMA
+    // than narrow tiles' MMAs take)
+    if (rank == 0) {
       pdl_wait();  // so that the bounded waits below do not count the previous kernel's time
+      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(width >> 3) << 17) |
+                             ((uint32_t)(2 * I8_M >> 4) << 24);
+      const uint64_t da0 = sw128_desc(ring_s), db0 = sw128_desc(ring_s + I8_ABYTES);
       bool ok = true;
       int s = 0, t = 0;
       uint32_t phase = 0u;
       for (; t < mine && ok; ++t) {
         const int b = t & 1;
         if (t >= 2) ok = mbar_wait(saddr(&tempty[b]), (uint32_t)((t / 2 - 1) & 1), &abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         for (int k = 0; k < p.nk && ok; ++k) {
           ok = mbar_wait(saddr(&full[s]), phase, &abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = sw128_desc(ring_s + s * PR_STAGE), db = sw128_desc(ring_s + s * PR_STAGE + I8_ABYTES);
+          if (elect_one()) {
+            const uint64_t da = da0 + (uint64_t)(s * (PR_STAGE / 16)), db = db0 + (uint64_t)(s * (PR_STAGE / 16));
 #pragma unroll
-          for (int kk = 0; kk < I8_KB / 32; ++kk)
-            tc_mma_i8<2>(tmem + b * PR_N, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), PR_IDESC,
-                         k > 0 || kk > 0);
-          tc_commit_pair(saddr(&empty[s]));
+            for (int kk = 0; kk < I8_KB / 32; ++kk)
+              tc_mma_i8<2>(tmem + b * PR_N, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), idesc,
+                           k > 0 || kk > 0);
+            tc_commit_pair(saddr(&empty[s]));
+          }
+          __syncwarp();
           if (++s == PR_S) {
             s = 0;
             phase ^= 1u;
           }
         }
-        if (ok) tc_commit_pair(saddr(&tfull[b]));
+        if (ok && elect_one()) tc_commit_pair(saddr(&tfull[b]));
+        __syncwarp();
       }
       // no MMA outlives the pair's operands or accumulators: the last commit
-      if (ok && mine > 0) mbar_wait_drain(saddr(&tfull[(mine - 1) & 1]), (uint32_t)(((mine - 1) / 2) & 1));
-      else if (!ok) {
-        tc_commit_pair(saddr(&tfull[t & 1]));
+      if (ok && mine > 0) {
+        mbar_wait_drain(saddr(&tfull[(mine - 1) & 1]), (uint32_t)(((mine - 1) / 2) & 1));
+      } else if (!ok) {
+        if (elect_one()) tc_commit_pair(saddr(&tfull[t & 1]));
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000) {  // a launch that gave up: what was issued ends within microseconds
         }
@@ -556,7 +575,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
     for (int t = 0; t < mine; ++t) {
       const int tile = pair + t * pairs, b = t & 1;
       const int m = (tile / ntn) * 2 * I8_M + (int)rank * I8_M + quarter * 32 + lane;
-      const int n0 = (tile % ntn) * PR_N + half * (PR_N / 2), nn = min(PR_N / 2, p.N - n0);
+      const int n0 = (tile % ntn) * width + half * hw, nn = min(hw, p.N - n0);
       __syncwarp();
       for (int c = lane; c < nn; c += 32) xs[c] = p.xs[n0 + c];
       const float ws = m < p.M ? p.ws[m] : 0.0f, bv = m < p.M && p.bias ? p.bias[m] : 0.0f;
@@ -564,7 +583,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       if (!mbar_wait(saddr(&tfull[b]), (uint32_t)((t / 2) & 1), &abort_flag)) break;
       __syncwarp();
       tc_fence_after();
-      store_cols<Y, PR_N / 2>(tmem + ((uint32_t)(quarter * 32) << 16) + b * PR_N + half * (PR_N / 2), nn, xs, ws, bv,
+      store_cols<Y, PR_N / 2>(tmem + ((uint32_t)(quarter * 32) << 16) + b * PR_N + half * hw, nn, xs, ws, bv,
                               static_cast<Y*>(p.y) + (int64_t)n0 * p.ldy + m - lane, p.ldy, p.M - m + lane, lane);
       tc_fence_before();
       __syncwarp();
@@ -638,20 +657,35 @@ template <typename Y>
 int launch_pair(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t st) {
   if (int rc = allow_max_smem((const void*)k_int8_pair<Y>, dev)) return rc;
   const int64_t mt = (c.M + 2 * I8_M - 1) / (2 * I8_M);
-  const int64_t step = std::max<int64_t>(1, (((int64_t)1 << 30) / mt)) * PR_N;  // tiles of one launch below 2^30
+  const int64_t step = std::max<int64_t>(1, (((int64_t)1 << 30) / mt)) * 32;  // tiles of one launch below 2^30
+  const int most = dev.sms / 2;
   for (int64_t n0 = 0; n0 < c.N; n0 += step) {
-    const int64_t n = std::min(step, c.N - n0), ntn = (n + PR_N - 1) / PR_N;
+    const int64_t n = std::min(step, c.N - n0);
+    // the tile width whose rounds over the pairs cost least: a tile's time is that
+    // of its width and about 140 columns more (4096 tokens, 4096 -> 22016: 8.0 us
+    // a round of 128 columns, 11.8 of 256; 1000 tokens, 2064 -> 5003: 80 tiles of
+    // 256 in two rounds take 24 us, 120 of 192 in two 21)
+    int width = PR_N;
+    int64_t cost = -1;
+    for (int w = PR_N; w >= 32; w -= 32) {
+      const int64_t rounds = (mt * ((n + w - 1) / w) + most - 1) / most, cw = rounds * (w + 140);
+      if (cost < 0 || cw < cost) {
+        cost = cw;
+        width = w;
+      }
+    }
+    const int64_t ntn = (n + width - 1) / width;
     if (int rc = encode_tensor_2d(&a.wmap, false, c.wq, c.K, c.M, c.ldw, I8_KB, I8_M, true)) return rc;
     if (int rc = encode_tensor_2d(&a.xmap, false, static_cast<const int8_t*>(c.xq) + n0 * c.ldx, c.K, n,
-                                  c.ldx, I8_KB, PR_N / 2, true))
+                                  c.ldx, I8_KB, width / 2, true))
       return rc;
     a.xs = c.xs + n0;
     a.y = static_cast<Y*>(c.y) + n0 * c.ldy;
     a.N = (int)n;
     const int64_t tiles = mt * ntn;
-    const int pairs = (int)std::min<int64_t>(tiles, dev.sms / 2);
+    const int pairs = (int)std::min<int64_t>(tiles, most);
     // the cluster size is the kernel's own
-    if (int rc = launch("k_int8_pair", k_int8_pair<Y>, dim3(2 * pairs), PR_THREADS, PR_SMEM, 0, st, a, (int)ntn,
+    if (int rc = launch("k_int8_pair", k_int8_pair<Y>, dim3(2 * pairs), PR_THREADS, PR_SMEM, 0, st, a, width, (int)ntn,
                         (int)tiles))
       return rc;
   }
@@ -663,9 +697,10 @@ int matmul_as(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
   if (c.N <= 16) return launch_mm<16, Y>(c, a, dev, st);
   if (c.N <= 32) return launch_mm<32, Y>(c, a, dev, st);
   if (c.N <= 64) return launch_mm<64, Y>(c, a, dev, st);
-  // pairs where their tiles fill the device, else tiles of 128 x 128
-  const int64_t tiles = ((c.M + 2 * I8_M - 1) / (2 * I8_M)) * ((c.N + PR_N - 1) / PR_N);
-  if (tiles < dev.sms / 2) return launch_mm<128, Y>(c, a, dev, st);
+  // up to 128 tokens single CTAs (100 tokens, 4096 -> 22016: 22 us against 28 in
+  // pairs; 128 tokens, 4096 -> 4096: 12 and 13.5), above that pairs (129 tokens
+  // 17 and 14, 512 tokens 30 and 15)
+  if (c.N <= 128) return launch_mm<128, Y>(c, a, dev, st);
   return launch_pair<Y>(c, a, dev, st);
 }
 

@@ -91,6 +91,13 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t d, uint64_t a, uint64_t b, ui
         : "memory");
 }
 
+// One lane of a converged warp: the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 // 32 lanes x NC consecutive 32-bit TMEM columns.
 template <int NC>
 __device__ __forceinline__ void tmem_ld(uint32_t ta, uint32_t (&v)[NC]) {

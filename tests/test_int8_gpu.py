@@ -226,20 +226,25 @@ def test_captured_replayed_and_on_two_streams():
 def test_a_wait_that_runs_out_is_reported():
     lib = _lib.lib()
     g = torch.Generator(DEV).manual_seed(3)
-    wq, ws = qg.quantize_int8(torch.randn(8192, 8192, device=DEV, generator=g))
-    xs = [torch.randn(n, 8192, device=DEV, generator=g) for n in (1, 500)]
-    want = [qg.int8_linear(x, wq, ws) for x in xs]
-    torch.cuda.synchronize()
-    for x, w in zip(xs, want):
-        assert lib.qgemv_set_wait_limit(1) == 0  # shorter than the ring's own waits
-        try:
-            qg.int8_linear(x, wq, ws)
-            torch.cuda.synchronize()
-        finally:
-            assert lib.qgemv_set_wait_limit(0) == 0
-        assert lib.qgemv_check_device_error(1, None) == 6
+    wq, ws = qg.quantize_int8(torch.randn(16384, 8192, device=DEV, generator=g))
+    for n in (1, 500):  # single CTAs, CTA pairs
+        xq, xs = qg.quantize_int8(torch.randn(n, 8192, device=DEV, generator=g))
+        want = qg.int8_matmul(xq, xs, wq, ws)
+        torch.cuda.synchronize()
+        seen = False
+        for _ in range(20):
+            assert lib.qgemv_set_wait_limit(1) == 0  # 1 us: shorter than a DRAM round trip under load
+            try:
+                qg.int8_matmul(xq, xs, wq, ws)
+                torch.cuda.synchronize()
+            finally:
+                assert lib.qgemv_set_wait_limit(0) == 0
+            if lib.qgemv_check_device_error(1, None) == 6:
+                seen = True
+                break
+        assert seen, "no wait ran out under a 1 us limit"
         assert lib.qgemv_check_device_error(0, None) == 0
-        assert torch.equal(qg.int8_linear(x, wq, ws), w)
+        assert torch.equal(qg.int8_matmul(xq, xs, wq, ws), want)
     assert lib.qgemv_check_device_error(0, None) == 0
 
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import qgemv_roofline_b200 as qg
+from qgemv_roofline_b200 import _lib
 from oracle import qformats_oracle as o
 
 import moe_reference as ref
@@ -323,6 +324,33 @@ def test_two_streams_at_once():
     qg.moe_layer(xs[1], r, L.experts, 4, y=y, stream=streams[0].cuda_stream)
     streams[0].synchronize()
     assert torch.equal(y, want[1])
+
+
+def test_a_wait_that_runs_out_is_reported():
+    lib = _lib.lib()
+    L = Layer(8, 1024, 2048, "q8_0", seed=23)
+    x, x64 = L.x(16)
+    ids, w = choose(L.rng, 16, 8, 2)
+    args = x, gpu(ids), gpu(w), L.experts
+    want = qg.moe_experts(*args)
+    torch.cuda.synchronize()
+    flush = torch.empty(64 << 20, device=DEV)  # the weights leave L2
+    seen = False
+    for _ in range(30):
+        flush.zero_()
+        assert lib.qgemv_set_wait_limit(1) == 0  # 1 us: shorter than a DRAM round trip under load
+        try:
+            qg.moe_experts(*args)
+            torch.cuda.synchronize()
+        finally:
+            assert lib.qgemv_set_wait_limit(0) == 0
+        if lib.qgemv_check_device_error(1, None) == 6:
+            seen = True
+            break
+    assert seen, "no wait ran out under a 1 us limit"
+    assert lib.qgemv_check_device_error(0, None) == 0
+    assert torch.equal(qg.moe_experts(*args), want)
+    assert lib.qgemv_check_device_error(0, None) == 0
 
 
 def test_experts_from_float_and_from_matrices():
