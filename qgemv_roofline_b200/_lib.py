@@ -220,7 +220,7 @@ def last_error() -> str:
 
 def call(name: str, *args) -> None:
     """Calls a status-returning entry point; raises QGemvError on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != OK:
         raise QGemvError(name, rc, last_error())
 

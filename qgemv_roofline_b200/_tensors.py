@@ -14,17 +14,26 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def on_device_of_x(fn):
     """Runs ``fn(x, ...)`` with the device of ``x`` current."""
     @functools.wraps(fn)
     def wrapper(x, *args, **kwargs):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        index = x.get_device() if isinstance(x, torch.Tensor) else -1
+        if index < 0:
             raise ValueError("x must be a CUDA tensor")
-        if x.get_device() == torch.cuda.current_device():
+        if index == _current_device():
             return fn(x, *args, **kwargs)
-        with torch.cuda.device(x.device):
+        with torch.cuda.device(index):
             return fn(x, *args, **kwargs)
     return wrapper
+
+
+def new(shape, dtype, device) -> torch.Tensor:
+    """An uninitialised contiguous tensor [M] or [N, M] (two thirds of torch.empty's time)."""
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=device)
 
 
 def rows_of(x: torch.Tensor, K: int):
@@ -48,7 +57,7 @@ def rows_of(x: torch.Tensor, K: int):
 def out_for(y, shape, dtype, device, vec: bool):
     """The output rows [N, M] of a call: (tensor to return, row stride)."""
     if y is None:
-        return torch.empty(shape[1:] if vec else shape, dtype=dtype, device=device), shape[1]
+        return new(shape[1:] if vec else shape, dtype, device), shape[1]
     want = tuple(shape[1:] if vec else shape)
     if y.dtype != dtype or y.device != device or tuple(y.shape) != want:
         raise ValueError(f"y must be a {dtype} tensor {want} on {device}")

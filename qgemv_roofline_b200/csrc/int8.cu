@@ -78,15 +78,18 @@ template <typename T> __device__ __forceinline__ float as_f32(T v) { return (flo
 template <> __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// rint(x / s), the quotient rounded to fp32 first.  x * (1 / s) is within
-// 127 * 2^-22 of it, so only quotients that near to a tie (or any, where 1 / s
-// is not accurate) need the division itself.
-__device__ __forceinline__ int quant1(float v, float s, float inv, bool exact) {
-  const float r = v * inv;
-  float q = rintf(r);
-  if (exact || fabsf(fabsf(r - q) - 0.5f) < 6.2e-5f)
-    q = fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
-  return (int)q;
+// q = rint(x / s), the quotient rounded to fp32 first, in the low byte.  x * (1 / s)
+// is within 127 * 2^-22 of the quotient, so only where it comes that near to a
+// tie (or where 1 / s is not accurate) is the division itself needed.  Adding
+// 1.5 * 2^23 rounds to an integer, half to even, which is then the low bits of
+// the sum: no conversion instruction (16 a clock per SM, and there were two).
+__device__ __forceinline__ uint32_t quant_near(float v, float inv, bool& tie) {
+  const float r = v * inv, t = r + 12582912.0f;
+  tie |= fabsf(fabsf(r - (t - 12582912.0f)) - 0.5f) < 6.2e-5f;
+  return __float_as_uint(t);
+}
+__device__ __noinline__ uint32_t quant_exact(float v, float s) {
+  return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
 }
 
 constexpr int RQ_THREADS = 256;
@@ -152,8 +155,16 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
     auto put8 = [&](const Raw& v, int i) {
       uint32_t w[2] = {0u, 0u};
       if (some) {
+        uint32_t b[8];
+        bool tie = exact;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(quant1(value(v, j), sc, inv, exact) & 0xFF) << (8 * (j & 3));
+        for (int j = 0; j < 8; ++j) b[j] = quant_near(value(v, j), inv, tie);
+        if (tie)
+          for (int j = 0; j < 8; ++j) b[j] = quant_exact(value(v, j), sc);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040),
+                             0x5410);
       }
       reinterpret_cast<uint2*>(qr)[i] = make_uint2(w[0], w[1]);
     };
@@ -169,7 +180,7 @@ __global__ void __launch_bounds__(RQ_THREADS) k_quant_rows(const T* __restrict__
     }
   } else {
     for (int k = threadIdx.x; k < K; k += RQ_THREADS)
-      qr[k] = some ? (int8_t)quant1(as_f32(xr[k]), sc, inv, exact) : (int8_t)0;
+      qr[k] = some ? (int8_t)quant_exact(as_f32(xr[k]), sc) : (int8_t)0;
   }
 }
 

@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from ._tensors import DTYPE_CODE, on_device_of_x, out_for, rows_of, stream_of, workspace
+from ._tensors import DTYPE_CODE, new, on_device_of_x, out_for, rows_of, stream_of, workspace
 
 
 @on_device_of_x
@@ -37,7 +37,7 @@ def quantize_int8(x: torch.Tensor, q: torch.Tensor | None = None, scales: torch.
     X, N, ldx, code = rows_of(x, K)
     vec = x.dim() == 1
     if q is None:
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        q = new(x.shape, torch.int8, x.device)
     elif q.dtype != torch.int8 or q.shape != x.shape or q.device != x.device or q.stride(-1) != 1 or \
             (not vec and N > 1 and q.stride(0) < K):
         raise ValueError("q must be an int8 tensor like x with unit last stride")
@@ -53,11 +53,12 @@ def quantize_int8(x: torch.Tensor, q: torch.Tensor | None = None, scales: torch.
 
 
 def _weights(wq, ws, bias, K, device):
-    if wq.dtype != torch.int8 or wq.dim() != 2 or wq.shape[1] != K or wq.device != device or \
+    shape = wq.shape
+    if wq.dtype != torch.int8 or len(shape) != 2 or shape[1] != K or wq.get_device() != device.index or \
             wq.stride(1) != 1:
         raise ValueError(f"wq must be an int8 tensor [M, K={K}] with unit last stride on {device}")
-    M = wq.shape[0]
-    if ws.dtype != torch.float32 or ws.shape != (M,) or ws.device != device or not ws.is_contiguous():
+    M = shape[0]
+    if ws.dtype != torch.float32 or ws.shape != (M,) or ws.get_device() != device.index or not ws.is_contiguous():
         raise ValueError(f"ws must be a contiguous float32 tensor [{M}] on {device}")
     if bias is None:
         return M, None
@@ -84,14 +85,15 @@ def int8_matmul(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.
     float32 [M], bias float32 [M].  K is a multiple of 16 below 2^17; rows start on 16-byte
     boundaries (any such row stride).
     """
-    if xq.dtype != torch.int8 or xq.dim() not in (1, 2) or (xq.stride(-1) != 1 and xq.shape[-1] > 1):
+    shape = xq.shape
+    if xq.dtype != torch.int8 or len(shape) not in (1, 2) or (xq.stride(-1) != 1 and shape[-1] > 1):
         raise ValueError("xq must be an int8 tensor [K] or [N, K] with unit last stride")
-    vec = xq.dim() == 1
-    N, K = (1, xq.shape[0]) if vec else xq.shape
+    vec = len(shape) == 1
+    N, K = (1, shape[0]) if vec else shape
     device = xq.device
-    if xs.dtype != torch.float32 or xs.shape != xq.shape[:-1] or xs.device != device or \
+    if xs.dtype != torch.float32 or xs.shape != shape[:-1] or xs.get_device() != device.index or \
             not xs.is_contiguous():
-        raise ValueError(f"xs must be a contiguous float32 tensor {tuple(xq.shape[:-1])} on {device}")
+        raise ValueError(f"xs must be a contiguous float32 tensor {tuple(shape[:-1])} on {device}")
     M, b = _weights(wq, ws, bias, K, device)
     code = _y_code(out_dtype)
     y, ldy = out_for(y, (N, M), out_dtype, device, vec)

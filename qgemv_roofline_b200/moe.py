@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from ._tensors import DTYPE_CODE, on_device_of_x, out_for, rows_of, stream_of, workspace
+from ._tensors import DTYPE_CODE, new, on_device_of_x, out_for, rows_of, stream_of, workspace
 from .gemv import QuantizedMatrix
 from .qformats import BLOCK_BYTES, QK
 
@@ -29,19 +29,21 @@ MAX_EXPERTS, MAX_CHOICES = 1024, 32
 
 
 def _router(router, top_k, scoring, bias, scale, normalize, device) -> _lib.MoeRouter:
-    if router.dim() != 2 or router.device != device or router.dtype not in DTYPE_CODE:
+    shape, code = router.shape, DTYPE_CODE.get(router.dtype)
+    if len(shape) != 2 or code is None or router.get_device() != device.index:
         raise ValueError(f"router must be a float32, bfloat16 or float16 tensor [E, K] on {device}")
-    if router.stride(1) != 1 or (router.shape[0] > 1 and router.stride(0) < router.shape[1]):
+    ldw, last = router.stride()
+    E = shape[0]
+    if last != 1 or (E > 1 and ldw < shape[1]):
         raise ValueError("router must have unit last stride and rows that do not overlap")
     if scoring not in SCORING:
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    E = router.shape[0]
     if not 1 <= top_k <= min(E, MAX_CHOICES):
         raise ValueError(f"top_k must be in [1, min(E={E}, {MAX_CHOICES})], got {top_k}")
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)
                              or bias.device != device or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous float32 tensor [{E}] on {device}")
-    return _lib.MoeRouter(router.data_ptr(), DTYPE_CODE[router.dtype], E, router.stride(0),
+    return _lib.MoeRouter(router.data_ptr(), code, E, ldw,
                           None if bias is None else bias.data_ptr(), top_k, SCORING[scoring],
                           bool(normalize), scale)
 
@@ -63,8 +65,7 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, *, scoring: str
     device = x.device
     r = _router(router, top_k, scoring, bias, scale, normalize, device)
     shape = (N, top_k) if x.dim() == 2 else (top_k,)
-    ids = torch.empty(shape, dtype=torch.int32, device=device)
-    weights = torch.empty(shape, dtype=torch.float32, device=device)
+    ids, weights = new(shape, torch.int32, device), new(shape, torch.float32, device)
     _lib.call("qgemv_moe_route", ctypes.byref(r), X.data_ptr(), code, ldx, N, X.shape[-1],
               ids.data_ptr(), weights.data_ptr(), stream_of(stream, device))
     return ids, weights
@@ -189,7 +190,8 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     slots = ids.shape[-1] if ids.dim() else 0
     want = (slots,) if vec else (N, slots)
     if (ids.shape != want or weights.shape != want or ids.dtype != torch.int32
-            or weights.dtype != torch.float32 or ids.device != device or weights.device != device
+            or weights.dtype != torch.float32 or ids.get_device() != device.index
+            or weights.get_device() != device.index
             or not ids.is_contiguous() or not weights.is_contiguous()):
         raise ValueError(f"ids (int32) and weights (float32) must be contiguous [N={N}, slots] on {device}")
     if not 1 <= slots <= MAX_CHOICES:
