@@ -9,7 +9,7 @@
 // Three launches, chained by programmatic dependent launch (no kernel waits on
 // another's blocks, no counters, no atomics on global memory):
 //
-//  * k_moe_route: one cluster of 8 CTAs per 8 tokens; logits in 64-bit sums,
+//  * k_moe_route: a cluster of CTAs per 1, 2 or 16 tokens; logits in 64-bit sums,
 //    rounded to fp32 once (so the choice of experts does not depend on the
 //    order of the sum), exchanged through distributed shared memory, then the
 //    top k of each token by one warp.  Further CTAs of the same launch round x
@@ -26,7 +26,17 @@
 // fills a ring of 9 stages with bulk copies (a stage is a slab: 4 row tiles x 2
 // or 4 groups of 128 columns, 17 or 18 KB in one contiguous piece), and 12
 // compute warps, one per row tile and one of three splits: split s takes every
-// third slab.  Every wait is bounded.
+// third slab.  Every wait is bounded.  What bounds them (one B200; the copy rate
+// is 6.54 TB/s): with few tokens per expert q8_0 the weights' stream (16 tokens,
+// 64 + 2 experts of 4096x1408: 971 MB in 178 us, 0.83 of the copy rate); q4_0 with
+// several tokens the instructions per 16 x 32 weights (42 against the 50 that the
+// stream leaves room for, at 0.6 to 0.8 issued per cycle: 64 tokens, 128 experts of
+// 2048x768, 335 MB in 105 us, 0.49); a single token the launches' latencies (128
+// experts of 2048x768 in q4_0, 8 chosen, 22 MB: 20 us, of which routing 8, entries
+// and first copies 2 x 2, the two products' slabs 5).  Tried and slower: 16 compute
+// warps of 96 registers (64 tokens 105 -> 156 us, spills), four MMAs of tokens per
+// entry (spills), units of their own for the splits (64 tokens 105 -> 103 us, one
+// token 20 -> 22), private rings of 16 warps without a producer (149 us).
 //
 // The arithmetic is the library's exact-integer scheme.  A block of 32
 // activations is rounded to integers X = rint(x FX / max |x|) and split into
@@ -512,8 +522,8 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
 constexpr int RM_TN = 16, RM_CL = 8, RM_TE = 16;
 // Four columns of a row as they were read: a row that can be read in vectors
 // keeps its type until it is used, so that the loads of the next steps are in
-// flight meanwhile (converted at once, each step waited for its loads: 120 us
-// instead of @@512 below).
+// flight meanwhile (converted at once, each step waited for its loads: 512 tokens,
+// 256 experts of 4096 columns took 120 us, now 60).
 struct Raw4 {
   uint32_t v[4];
   __device__ __forceinline__ void load(const void* p, int dt, int64_t i, int n, bool vec) {
@@ -1544,7 +1554,7 @@ int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const Dev
                  cudaStream_t st) {
   // up to 32 tokens two to a cluster (latency counts: the clusters run side by
   // side), above that sixteen on matrix instructions (512 tokens, 256 experts of
-  // 4096 columns: 8 tokens a cluster on DFMA 230 us, @@512)
+  // 4096 columns: 8 tokens a cluster on DFMA 230 us, now 60)
   if (a.N == 1) return launch_route_n<1>(a, r, route, prep, dev, st);
   if (a.N <= 32) return launch_route_n<2>(a, r, route, prep, dev, st);
   r.clusters = route ? (a.N + RM_TN - 1) / RM_TN : 0;

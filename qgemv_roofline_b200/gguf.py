@@ -170,6 +170,23 @@ class GGUFReader:
         return QuantizedMatrix(fmt, M, nb * 32, "soa", q=q, d=d)
 
 
+    def load_experts(self, gate: str, up: str, down: str, device="cuda", n_shared: int = 0):
+        """Three expert tensors (ggml dims (K, F, E), (K, F, E) and (F, K, E)) as
+        ``QuantizedExperts`` on ``device``."""
+        import torch
+
+        from .moe import QuantizedExperts
+
+        dims = [self.tensors[n].dims for n in (gate, up, down)]
+        if any(len(d) != 3 for d in dims) or dims[0] != dims[1] or \
+                dims[2] != (dims[0][1], dims[0][0], dims[0][2]):
+            raise ValueError(f"{gate}, {up}, {down}: expert tensors of dims (K, F, E), (K, F, E) and "
+                             f"(F, K, E), got {dims}")
+        with torch.cuda.device(device):
+            return QuantizedExperts.from_matrices(*[self.load(n, device) for n in (gate, up, down)],
+                                                  n_experts=dims[0][2], n_shared=n_shared)
+
+
 def _put_value(out: bytearray, v):
     if isinstance(v, bool):
         out += struct.pack("<I?", T_BOOL, v)
@@ -201,8 +218,8 @@ def _put_value(out: bytearray, v):
 def write_gguf(path: str, tensors: dict, metadata: dict | None = None, alignment: int = 32):
     """Writes a GGUF version 3 file.
 
-    ``tensors`` maps names to ``("q8_0" | "q4_0", blocks uint8 [rows, K/32, 34|18])`` or to
-    float32 / float16 numpy arrays (torch order).  ``metadata`` values may be bool, int,
+    ``tensors`` maps names to ``("q8_0" | "q4_0", blocks uint8 [rows, K/32, 34|18])`` (or
+    [experts, rows, K/32, 34|18]) or to float32 / float16 numpy arrays (torch order).  ``metadata`` values may be bool, int,
     float, str or lists of one of those.
     """
     meta = dict(metadata or {})
@@ -213,9 +230,9 @@ def write_gguf(path: str, tensors: dict, metadata: dict | None = None, alignment
             fmt, blk = v
             blk = np.ascontiguousarray(blk, dtype=np.uint8)
             t = {"q8_0": GGML_Q8_0, "q4_0": GGML_Q4_0}[fmt]
-            if blk.ndim != 3 or blk.shape[2] != _BLOCK[t][1]:
+            if blk.ndim not in (3, 4) or blk.shape[-1] != _BLOCK[t][1]:
                 raise ValueError(f"{name}: blocks must be [rows, K/32, {_BLOCK[t][1]}]")
-            dims = (blk.shape[1] * 32, blk.shape[0])
+            dims = (blk.shape[-2] * 32, *reversed(blk.shape[:-2]))
             data = blk.tobytes()
         else:
             arr = np.ascontiguousarray(v)

@@ -373,6 +373,30 @@ def test_experts_from_float_and_from_matrices():
     assert (np.abs(y.double().cpu().numpy() - want) <= tol).all()
 
 
+def test_experts_from_a_gguf_file(tmp_path):
+    from qgemv_roofline_b200 import gguf
+    E, K, F = 3, 96, 64
+    rng = np.random.default_rng(4)
+    parts = {"gate": ("q4_0", planes("q4_0", E, F, K, rng)), "up": ("q4_0", planes("q4_0", E, F, K, rng)),
+             "down": ("q8_0", planes("q8_0", E, K, F, rng))}
+    tensors = {}
+    for name, (fmt, (q, d)) in parts.items():
+        rows = q.shape[1]
+        b = qg.to_aos(fmt, torch.from_numpy(q.reshape(E * rows, -1)), torch.from_numpy(d.reshape(E * rows, -1)))
+        tensors[f"blk.0.ffn_{name}_exps.weight"] = (fmt, b.numpy().reshape(E, rows, *b.shape[1:]))
+    path = str(tmp_path / "experts.gguf")
+    gguf.write_gguf(path, tensors)
+    names = list(tensors)
+    r = gguf.GGUFReader(path)
+    assert r.tensors[names[0]].dims == (K, F, E) and r.tensors[names[2]].dims == (F, K, E)
+    a = r.load_experts(*names)
+    with pytest.raises(ValueError):
+        r.load_experts(names[0], names[2], names[1])
+    b = qg.QuantizedExperts(*[(gpu(q), gpu(d)) for _, (q, d) in parts.values()])
+    assert torch.equal(a.gate_up, b.gate_up) and torch.equal(a.down, b.down)
+    assert (a.n_experts, a.hidden, a.ffn, a.fmt, a.fmt_down) == (E, K, F, "q4_0", "q8_0")
+
+
 def test_refusals():
     L = Layer(4, 64, 32, "q8_0", shared=1, seed=30)
     x, _ = L.x(2)
