@@ -328,17 +328,15 @@ def test_two_streams_at_once():
 
 def test_a_wait_that_runs_out_is_reported():
     lib = _lib.lib()
-    L = Layer(8, 1024, 2048, "q8_0", seed=23)
-    x, x64 = L.x(16)
-    ids, w = choose(L.rng, 16, 8, 2)
+    L = Layer(4, 8192, 256, "q8_0", seed=23)  # half a megabyte per unit: its sums come microseconds late
+    x, x64 = L.x(4)
+    ids, w = choose(L.rng, 4, 4, 2)
     args = x, gpu(ids), gpu(w), L.experts
     want = qg.moe_experts(*args)
     torch.cuda.synchronize()
-    flush = torch.empty(64 << 20, device=DEV)  # the weights leave L2
     seen = False
     for _ in range(30):
-        flush.zero_()
-        assert lib.qgemv_set_wait_limit(1) == 0  # 1 us: shorter than a DRAM round trip under load
+        assert lib.qgemv_set_wait_limit(1) == 0
         try:
             qg.moe_experts(*args)
             torch.cuda.synchronize()
