@@ -584,7 +584,7 @@ QGEMV_API size_t qgemv_moe_workspace_bytes(int64_t n_tokens, int32_t slots, int6
  * [0, n_experts): no expert, e.g. -1; the same expert twice: the sum of its
  * weights), weights fp32 [N][slots].  A token without an expert gets zeros.
  * n_shared is not used here.  workspace NULL: the stream's (allocated by the
- * first such call, outside stream capture); else 16-byte aligned. */
+ * first such call; refused under stream capture); else 16-byte aligned. */
 QGEMV_API int qgemv_moe_experts(const qgemv_expert_set* experts, const void* x, int dtype,
                                 int64_t ldx, const int32_t* ids, const float* weights,
                                 int32_t slots, int64_t n_tokens, void* y, int64_t ldy,
@@ -620,7 +620,7 @@ QGEMV_API int qgemv_int8_matmul(const void* xq, const float* xs, int64_t ldx, co
                                 void* stream);
 /* The two together: x (fp32, bf16 or fp16) is rounded per token into the
  * workspace (16-byte aligned; NULL: the stream's, allocated by the first such
- * call outside stream capture), then multiplied. */
+ * call and refused under stream capture), then multiplied. */
 QGEMV_API size_t qgemv_int8_linear_workspace_bytes(int64_t N, int64_t K);
 QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const void* wq,
                                 const float* ws, int64_t ldw, const float* bias, int64_t N,

@@ -878,6 +878,21 @@ QGEMV_API int qgemv_moe_tile(int format, const void* q, const void* d, const voi
 }
 
 namespace {
+// The stream's workspace for a call that brought none.  Refused under capture:
+// a graph would keep the buffer's address, which a later, larger call on the
+// stream frees, and graphs captured on one stream would share it.
+int own_workspace(cudaStream_t st, size_t need, void** ws) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(st, &cs);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(ERR_CUDA, "cudaStreamIsCapturing: %s", cudaGetErrorString(e));
+  }
+  if (cs != cudaStreamCaptureStatusNone)
+    return set_error(ERR_UNSUPPORTED, "a captured call needs a workspace of its own (%zu bytes)", need);
+  return stream_workspace(st, need, ws);
+}
+
 int check_moe_x(const void* x, int dtype, int64_t ldx, int64_t N, int64_t K) {
   if (dtype < 0 || dtype > 2) return set_error(ERR_ARG, "dtype must be 0, 1 or 2, got %d", dtype);
   if (N < 0 || K < 1) return set_error(ERR_SHAPE, "n_tokens=%lld hidden=%lld", (long long)N, (long long)K);
@@ -957,7 +972,7 @@ int moe_entry(const qgemv_expert_set* m, const qgemv_moe_router* router, const v
     if (ws_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, ws_bytes);
     if (misaligned(ws, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = stream_workspace(st, need, &ws)) {
+  } else if (int rc = own_workspace(st, need, &ws)) {
     return rc;
   }
   MoeExperts e;
@@ -1025,8 +1040,8 @@ int check_int8_sizes(int64_t N, int64_t M, int64_t K) {
   if (K > kInt8MaxK)
     return set_error(ERR_UNSUPPORTED, "K=%lld: int32 sums are exact up to K=%lld", (long long)K,
                      (long long)kInt8MaxK);
-  if (N >= kMaxDim || M >= kMaxDim - 128)
-    return set_error(ERR_UNSUPPORTED, "N and M must be below 2^31 (N=%lld M=%lld)", (long long)N, (long long)M);
+  if (N >= kMaxDim - 512 || M >= kMaxDim - 512)  // tile origins stay in 32 bits
+    return set_error(ERR_UNSUPPORTED, "N and M must be below 2^31 - 512 (N=%lld M=%lld)", (long long)N, (long long)M);
   return OK;
 }
 
@@ -1109,7 +1124,7 @@ QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const voi
     if (workspace_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
     if (misaligned(workspace, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = stream_workspace(st, need, &workspace)) {
+  } else if (int rc = own_workspace(st, need, &workspace)) {
     return rc;
   }
   float* xs = static_cast<float*>(workspace);

@@ -202,6 +202,11 @@ def test_route_types_and_strides(dtype, rdtype):
     assert torch.equal(i1, ids[2]) and torch.equal(w1, w[2])
 
 
+def test_route_without_tokens():
+    ids, w = qg.moe_route(torch.zeros(0, 64, device=DEV), torch.zeros(5, 64, device=DEV), 2)
+    assert ids.shape == w.shape == (0, 2)
+
+
 def test_route_ties_go_to_the_lower_index():
     rng = np.random.default_rng(12)
     r = rng.standard_normal((50, 64)).astype(np.float32)
@@ -302,6 +307,46 @@ def test_captured_and_replayed():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, want[0]) for _, out in graphs)
+
+
+FIRST_CALLS = """
+import torch, qgemv_roofline_b200 as qg
+g = torch.Generator("cuda").manual_seed(1)
+w = [torch.randn(4, *s, device="cuda", generator=g) for s in ((64, 128), (64, 128), (128, 64))]
+experts = qg.QuantizedExperts.from_float(*w, "q8_0")
+router = torch.randn(4, 128, device="cuda", generator=g)
+wq, ws = qg.quantize_int8(w[0][0])
+xs = [torch.randn(n, 128, device="cuda", generator=g) for n in (1, 9, 40, 200)]
+calls = lambda: [f(x) for x in xs for f in (lambda x: qg.moe_layer(x, router, experts, 2), lambda x: qg.int8_linear(x, wq, ws))]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, calls()))
+stream = torch.cuda.Stream()
+with torch.cuda.stream(stream):
+    graph = torch.cuda.CUDAGraph()
+    graph.capture_begin()
+    for f in (lambda s: qg.moe_layer(xs[0], router, experts, 2, stream=s), lambda s: qg.int8_linear(xs[0], wq, ws, stream=s)):
+        try:
+            f(stream.cuda_stream)
+            raise SystemExit("a raw stream under capture was not refused")
+        except qg.QGemvError as e:
+            assert e.status == 5, e
+    graph.capture_end()
+print("first calls ok")
+"""
+
+
+def test_first_calls_of_a_process_are_captured():
+    """Nothing that a first call sets up is missing under capture; a raw stream handle under
+    capture, which would get the stream's shared workspace, is refused."""
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "first calls ok" in r.stdout, r.stdout + r.stderr
 
 
 def test_two_streams_at_once():
