@@ -14,6 +14,7 @@
 #include <mutex>
 #include <map>
 #include <set>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -116,6 +117,36 @@ int occupancy(const void* func, const DeviceInfo& dev, int threads, size_t smem,
   std::lock_guard<std::mutex> lk(g_mu);
   g_occ[key] = occ;
   *out = occ;
+  return OK;
+}
+
+int active_clusters(const void* func, const DeviceInfo& dev, int threads, size_t smem, int cs, int* out) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int>, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  const auto key = std::make_tuple(func, dev.device, cs);
+  const auto it = known.find(key);
+  if (it != known.end()) {
+    *out = it->second;
+    return OK;
+  }
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cs);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, func, &cfg);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(ERR_CUDA, "resident clusters of %d: %s", cs, cudaGetErrorString(e));
+  }
+  *out = known[key] = n;
   return OK;
 }
 

@@ -197,6 +197,8 @@ struct I8Args {
   int early_w;     // the weights may be read before the dependency wait
 };
 
+constexpr int I8_CL = 8;  // CTAs of a cluster at most
+
 // BN tokens per tile; S ring stages.  kind::i8: s32 accumulators (bits 4-5 =
 // 2), A and B signed (bits 7-9, 10-12 = 1), both K-major, N >> 3 at bit 17,
 // M >> 4 at bit 24.
@@ -221,13 +223,36 @@ __device__ __forceinline__ void put_y2(__half* y, float a, float b) {
   *reinterpret_cast<__half2*>(y) = __floats2half2_rn(a, b);
 }
 
+// Four channels of one token, `room` of them exist; one store where `vec`.
+__device__ __forceinline__ void put_y4(float* y, const float (&f)[4], int room, bool vec) {
+  if (vec && room >= 4) {
+    *reinterpret_cast<float4*>(y) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < room) y[i] = f[i];
+  }
+}
+template <typename Y>
+__device__ __forceinline__ void put_y4(Y* y, const float (&f)[4], int room, bool vec) {
+  if (vec && room >= 4) {
+    __align__(8) Y h[4];
+    put_y2(h, f[0], f[1]);
+    put_y2(h + 2, f[2], f[3]);
+    *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(h);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < room) put_y(y + i, f[i]);
+  }
+}
+
 // NC accumulator columns (tokens) from `ta` on, this lane's channel: scaled and
 // stored; `nn` of them exist.  xs: their scales in shared memory.  y: token 0's
 // element of the warp's first channel; `room`: channels from there on.  With a
 // 16-bit type and even addresses a pair of lanes trades values, so that one
 // store writes two channels of one token in the even lane and of the next in the
-// odd one (4096 tokens, 4096 -> 22016: the stores, not the MMAs, set the pace at
-// one value a store).
+// odd one: half the stores of one value each, and no 2-byte ones.
 template <typename Y, int NC>
 __device__ __forceinline__ void store_cols(uint32_t ta, int nn, const float* xs, float ws, float b, Y* y,
                                            int64_t ldy, int room, int lane) {
@@ -387,18 +412,34 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
   }
   __syncwarp();
   if (cs > 1) {
+    // A warp joins one token's 128 channels, four a lane, all parts in flight at
+    // once: a part is another SM's shared memory, so each read is a long
+    // latency and few bytes (128 tokens, 4096 -> 11008: one value a thread at a
+    // time 30.6 us, now 16.5 with the same two CTAs a tile)
+    const int nn = min(BN, p.N - n0), m = m0 + 4 * lane, room = p.M - m;
+    float ws[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ws[i] = i < room ? p.ws[m + i] : 0.0f;
+      b[i] = i < room && p.bias ? p.bias[m + i] : 0.0f;
+    }
+    const bool vec = (reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(Y) - 1)) == 0 && (p.ldy & 3) == 0;
+    const int4* part[I8_CL];
+#pragma unroll
+    for (int r = 0; r < I8_CL; ++r)
+      part[r] = reinterpret_cast<const int4*>(cl.map_shared_rank(reinterpret_cast<int*>(ring), min(r, cs - 1)));
     cl.sync();
-    if (warp >= 2) {
-      int* part = reinterpret_cast<int*>(ring);
-      const int row = (warp & 3) * 32 + lane, m = m0 + row, nn = min(BN, p.N - n0);
-      if (m < p.M) {
-        const float ws = p.ws[m], b = p.bias ? p.bias[m] : 0.0f;
-        for (int c = rank; c < nn; c += cs) {
-          int v = 0;
-          for (int r = 0; r < cs; ++r) v += cl.map_shared_rank(part, r)[c * I8_M + row];
-          put_y(y + (int64_t)(n0 + c) * p.ldy + m, fmaf((float)v * xs_s[c], ws, b));
-        }
-      }
+    for (int c = rank + cs * warp; c < nn; c += cs * (I8_THREADS / 32)) {
+      int4 v[I8_CL];
+#pragma unroll
+      for (int r = 0; r < I8_CL; ++r) v[r] = r < cs ? part[r][c * (I8_M / 4) + lane] : make_int4(0, 0, 0, 0);
+      int s[4] = {};
+#pragma unroll
+      for (int r = 0; r < I8_CL; ++r) s[0] += v[r].x, s[1] += v[r].y, s[2] += v[r].z, s[3] += v[r].w;
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = fmaf((float)s[i] * xs_s[c], ws[i], b[i]);
+      put_y4(y + (int64_t)(n0 + c) * p.ldy + m, f, room, vec);
     }
     cl.sync();  // no CTA leaves while another reads its part
   }
@@ -653,10 +694,23 @@ int launch_mm(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
     a.xs = c.xs + n0;
     a.y = static_cast<Y*>(c.y) + n0 * c.ldy;
     a.N = (int)n;
-    // few tiles: a cluster splits the K steps, as many CTAs as fit at once
-    const int per_sm = std::max(1, (int)((size_t)dev.smem_optin / C::SMEM));
+    // few tiles: a cluster splits the K steps, as many CTAs as are resident at
+    // once, each with enough steps that its part is worth the join: 2 at 16
+    // columns, up to 8 at 64 and more (4096 columns deep, clusters of 1/2/3/4/8:
+    // 64 tokens -> 11008 13.8/15.0/12.3/17.9/24.3 us, of which 4 and 8 are not
+    // resident; 128 tokens -> 4096 14.7/12.7/10.4/9.7/11.9)
+    const int least = std::min(8, BN / 8);
+    // by shared memory (2 KB for what is not dynamic): the occupancy query answers
+    // 1 for a kernel that allocates TMEM, though 3 ran at once at 16 columns
+    const int per_sm = std::max(1, (int)(dev.smem_optin / (C::SMEM + 2048)));
+    const int64_t room = (int64_t)per_sm * dev.sms / (tiles * nt);
     int cs = 1;
-    while (cs < 8 && tiles * nt * cs * 2 <= (int64_t)per_sm * dev.sms && a.nk >= cs * 4) cs *= 2;
+    for (int t = (int)std::min<int64_t>(std::min<int64_t>(I8_CL, room), a.nk / least); t > 1 && cs == 1; --t) {
+      int most = 0;
+      if (int rc = active_clusters((const void*)k_int8_mm<BN, Y>, dev, I8_THREADS, dev.smem_optin - 4096, t, &most))
+        return rc;  // with one CTA per SM
+      if (tiles * nt <= (int64_t)most * per_sm) cs = t;
+    }
     if (int rc = launch("k_int8_mm", k_int8_mm<BN, Y>, dim3(tiles * cs, (unsigned)nt), I8_THREADS, C::SMEM,
                         cs, st, a))
       return rc;

@@ -67,10 +67,8 @@
 // into the high half of a byte is 16 (n - 8) as a signed byte, one or two
 // instructions; the 1/16 is folded into the result's factor (exact).
 #include <algorithm>
-#include <map>
 #include <mutex>
 #include <set>
-#include <tuple>
 #include <utility>
 
 #include <cooperative_groups.h>
@@ -1476,38 +1474,6 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
     cudaGetLastError();
     return set_error(ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   }
-  return OK;
-}
-
-// Clusters of `cs` CTAs of a kernel that are resident at once (cached; kernels
-// that leave one CTA per SM whatever the call's shared memory).
-int active_clusters(const void* f, const DeviceInfo& dev, int threads, size_t smem, int cs, int* out) {
-  static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int>, int> known;
-  std::lock_guard<std::mutex> lk(mu);
-  const auto key = std::make_tuple(f, dev.device, cs);
-  const auto it = known.find(key);
-  if (it != known.end()) {
-    *out = it->second;
-    return OK;
-  }
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cs;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cs);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  int n = 0;
-  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, f, &cfg);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(ERR_CUDA, "resident clusters of %d: %s", cs, cudaGetErrorString(e));
-  }
-  *out = known[key] = n;
   return OK;
 }
 

@@ -30,6 +30,10 @@ int allow_max_smem(const void* func, const DeviceInfo& dev);
 // Resident blocks per SM of `func` (cached per device, block size and smem).
 int occupancy(const void* func, const DeviceInfo& dev, int threads, size_t smem, int* out);
 
+// Clusters of `cs` blocks of `func` that are resident at once with `smem` bytes
+// each, of which one block fits an SM (cached per device and cluster size).
+int active_clusters(const void* func, const DeviceInfo& dev, int threads, size_t smem, int cs, int* out);
+
 // All-gather fused into the single-column GEMV (one process per GPU): the
 // kernel also stores its rows into the other ranks' y buffers (peer
 // pointers) and the CTA that finishes last adds 1 to every rank's counter
