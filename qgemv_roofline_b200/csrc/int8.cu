@@ -15,10 +15,10 @@
 // past the end read as zeros.  TMEM lane = channel, column = token: a warp
 // stores 32 consecutive channels of a token at a time.  Two kernels:
 //
-//  * k_int8_mm (up to 128 tokens): one tile of 128 channels x 16 to 128 tokens per CTA
-//    or, where there are fewer tiles than CTAs, per cluster, whose CTAs split K
-//    and add their int32 parts through distributed shared memory (exact in any
-//    order).  With one token the weights' stream is what counts.
+//  * k_int8_mm (up to 128 tokens, more with few tiles): one tile of 128 channels
+//    x 16 to 128 tokens per CTA or, where the tiles leave room, per cluster, whose
+//    CTAs split K and add their int32 parts through distributed shared memory
+//    (exact in any order).  With one token the weights' stream is what counts.
 //  * k_int8_pair (more): persistent CTA pairs (tcgen05 cta_group::2) on tiles of
 //    256 channels x up to 256 tokens; each CTA copies its half of both operands, so
 //    that an SM reads 64 instead of 96 bytes of shared memory per cycle; two
@@ -678,6 +678,32 @@ int launch(const char* what, void (*f)(A...), dim3 grid, int threads, size_t sme
   return OK;
 }
 
+// With few tiles a cluster splits the K steps, as many CTAs as are resident at
+// once, each with enough steps that its part is worth the join: 2 at 16 columns,
+// up to 8 at 64 and more (4096 columns deep, clusters of 1/2/3/4/8: 64 tokens ->
+// 11008 13.8/15.0/12.3/17.9/24.3 us, of which 4 and 8 are not resident; 128
+// tokens -> 4096 14.7/12.7/10.4/9.7/11.9)
+template <int BN, typename Y>
+int split_of(int64_t tiles, int nk, const DeviceInfo& dev, int* cs) {
+  using C = I8Cfg<BN>;
+  const int least = std::min(8, BN / 8);
+  // by shared memory (2 KB for what is not dynamic): the occupancy query answers
+  // 1 for a kernel that allocates TMEM, though 3 ran at once at 16 columns
+  const int per_sm = std::max(1, (int)(dev.smem_optin / (C::SMEM + 2048)));
+  const int64_t room = (int64_t)per_sm * dev.sms / tiles;
+  *cs = 1;
+  for (int t = (int)std::min<int64_t>(std::min<int64_t>(I8_CL, room), nk / least); t > 1; --t) {
+    int most = 0;  // with one CTA per SM
+    if (int rc = active_clusters((const void*)k_int8_mm<BN, Y>, dev, I8_THREADS, dev.smem_optin - 4096, t, &most))
+      return rc;
+    if (tiles <= (int64_t)most * per_sm) {
+      *cs = t;
+      break;
+    }
+  }
+  return OK;
+}
+
 template <int BN, typename Y>
 int launch_mm(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t st) {
   using C = I8Cfg<BN>;
@@ -694,23 +720,8 @@ int launch_mm(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
     a.xs = c.xs + n0;
     a.y = static_cast<Y*>(c.y) + n0 * c.ldy;
     a.N = (int)n;
-    // few tiles: a cluster splits the K steps, as many CTAs as are resident at
-    // once, each with enough steps that its part is worth the join: 2 at 16
-    // columns, up to 8 at 64 and more (4096 columns deep, clusters of 1/2/3/4/8:
-    // 64 tokens -> 11008 13.8/15.0/12.3/17.9/24.3 us, of which 4 and 8 are not
-    // resident; 128 tokens -> 4096 14.7/12.7/10.4/9.7/11.9)
-    const int least = std::min(8, BN / 8);
-    // by shared memory (2 KB for what is not dynamic): the occupancy query answers
-    // 1 for a kernel that allocates TMEM, though 3 ran at once at 16 columns
-    const int per_sm = std::max(1, (int)(dev.smem_optin / (C::SMEM + 2048)));
-    const int64_t room = (int64_t)per_sm * dev.sms / (tiles * nt);
     int cs = 1;
-    for (int t = (int)std::min<int64_t>(std::min<int64_t>(I8_CL, room), a.nk / least); t > 1 && cs == 1; --t) {
-      int most = 0;
-      if (int rc = active_clusters((const void*)k_int8_mm<BN, Y>, dev, I8_THREADS, dev.smem_optin - 4096, t, &most))
-        return rc;  // with one CTA per SM
-      if (tiles * nt <= (int64_t)most * per_sm) cs = t;
-    }
+    if (int rc = split_of<BN, Y>(tiles * nt, a.nk, dev, &cs)) return rc;
     if (int rc = launch("k_int8_mm", k_int8_mm<BN, Y>, dim3(tiles * cs, (unsigned)nt), I8_THREADS, C::SMEM,
                         cs, st, a))
       return rc;
@@ -762,10 +773,20 @@ int matmul_as(const Int8Call& c, I8Args& a, const DeviceInfo& dev, cudaStream_t 
   if (c.N <= 16) return launch_mm<16, Y>(c, a, dev, st);
   if (c.N <= 32) return launch_mm<32, Y>(c, a, dev, st);
   if (c.N <= 64) return launch_mm<64, Y>(c, a, dev, st);
-  // up to 128 tokens single CTAs (100 tokens, 4096 -> 22016: 22 us against 28 in
-  // pairs; 128 tokens, 4096 -> 4096: 12 and 13.5), above that pairs (129 tokens
-  // 17 and 14, 512 tokens 30 and 15)
+  // Up to 128 tokens single CTAs (100 tokens, 4096 -> 22016: 21 us against 24 in
+  // pairs; 128 tokens, 4096 -> 4096: 9.7 and 12), above that pairs (129 tokens,
+  // 4096 -> 11008: 17 and 13.5; 512 tokens 29 and 22), but for few tiles that a
+  // cluster of 4 or more splits, with one CTA per SM (256 tokens, 4096 -> 1024: 8.2
+  // and 11.0) or a deep product (256 tokens, 11008 -> 4096: 18.3 and 22.9; 4096 ->
+  // 4096 12.1 and 11.6)
   if (c.N <= 128) return launch_mm<128, Y>(c, a, dev, st);
+  const int64_t tiles = (c.M + I8_M - 1) / I8_M * ((c.N + 127) / 128);
+  if (tiles * 4 <= dev.sms || (a.nk >= 64 && tiles * 2 <= dev.sms)) {
+    int cs = 1;
+    if (int rc = allow_max_smem((const void*)k_int8_mm<128, Y>, dev)) return rc;
+    if (int rc = split_of<128, Y>(tiles, a.nk, dev, &cs)) return rc;
+    if (cs >= 4) return launch_mm<128, Y>(c, a, dev, st);
+  }
   return launch_pair<Y>(c, a, dev, st);
 }
 

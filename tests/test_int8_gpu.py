@@ -63,6 +63,29 @@ def test_matmul(N, M, K, dtype, biased):
     check(y, *product(xq, xs, wq, ws, bias), dtype)
 
 
+@pytest.mark.parametrize("N,M,K", [
+    (1, 9000, 1040), (16, 6100, 2064), (31, 3331, 3120), (32, 11001, 1088), (64, 11006, 1040), (64, 2501, 4112),
+    (97, 4097, 2064), (127, 5003, 3088), (128, 8190, 1040), (129, 1001, 2576), (250, 1023, 4096), (257, 4000, 8208),
+    (640, 129, 1040), (513, 515, 8208)])
+@pytest.mark.parametrize("dtype", list(TORCH))
+@pytest.mark.parametrize("shift,pad", [(0, 0), (1, 2), (4, 4)])
+def test_splits_of_k(N, M, K, dtype, shift, pad):
+    """Clusters of every size, into rows of y that start at any element and hold more
+    than the product: what is beside it stays."""
+    rng = np.random.default_rng(N * M + K)
+    xq, wq = (torch.from_numpy(rng.integers(-128, 128, s, dtype=np.int8)).to(DEV) for s in ((N, K), (M, K)))
+    xs, ws = (torch.from_numpy(rng.random(n).astype(np.float32) * 1e-2).to(DEV) for n in (N, M))
+    bias = torch.from_numpy(rng.standard_normal(M).astype(np.float32)).to(DEV)
+    whole = torch.full((N, shift + M + pad), 77.0, dtype=TORCH[dtype], device=DEV)
+    y = whole[:, shift:shift + M]
+    qg.int8_matmul(xq, xs, wq, ws, bias, TORCH[dtype], y)
+    # integers below 2^53: exact in 64 bits in any order
+    want = (xq.double() @ wq.double().T) * xs.double()[:, None] * ws.double()
+    size = want.abs() + bias.double().abs()
+    check(y, (want + bias.double()).cpu().numpy(), size.cpu().numpy(), dtype)
+    assert (whole[:, :shift] == 77).all() and (whole[:, shift + M:] == 77).all()
+
+
 @pytest.mark.parametrize("N", [1, 40, 300])
 def test_sums_at_the_ends_of_int32(N):
     M, K = 130, 131056  # the largest K: 131056 * 128 * 128 = 2^31 - 2^18
