@@ -7,7 +7,8 @@
 //   y[n] = sum_j down_e h[n][j]
 //
 // Three launches, chained by programmatic dependent launch (no kernel waits on
-// another's blocks, no counters, no atomics on global memory):
+// another's blocks, no counters, no atomics on global memory; each reads global
+// memory only after its own dependency wait):
 //
 //  * k_moe_route: a cluster of CTAs per 1, 2 or 16 tokens; logits in 64-bit sums,
 //    rounded to fp32 once (so the choice of experts does not depend on the
@@ -1266,10 +1267,14 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
   float* ypart = reinterpret_cast<float*>(dn_smem + ring_bytes<FMT>());  // [split][token][64]
   const int yn = a.N * R;
   for (int i = threadIdx.x; i < MOE_KS * yn; i += DN_THREADS) ypart[i] = 0.0f;
-  // the choices were complete before k_moe_up passed its own wait and
-  // allowed this launch; what k_moe_up writes comes after the wait below
   uint8_t* const table = dn_smem + ring_bytes<FMT>() + (size_t)MOE_KS * yn * 4;
   clear_table(table, a);
+  // The choices are an earlier grid's writes too: that k_moe_up has waited for
+  // them orders nothing for this grid, whose SM may still hold an earlier call's.
+  // So nothing global is read before this grid's own wait, and no bounded wait
+  // (the producer's for empty stages) counts k_moe_up's time.
+  pdl_wait();
+  pdl_trigger();
   const Table tb = build_table<ent_tok<DIG>()>(table, a);
   const int fg = groups_of(a.F), fs = (fg + SG - 1) / SG, chunks = (a.K + R - 1) / R;
   const int64_t total = (int64_t)tb.nent * fs;
@@ -1289,10 +1294,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
       feed.finish();
     }
     __syncwarp();
-    pdl_wait();
   } else {
-    pdl_wait();
-    pdl_trigger();
     const int rt = warp % MOE_RT, kq = warp / MOE_RT;
     float* yp = ypart + kq * yn + rt * 16 + (lane >> 2);
     Work<FMT, DIG> w;
