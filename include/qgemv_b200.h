@@ -520,8 +520,9 @@ QGEMV_API int qgemv_mg_destroy(void* handle);
  *   y[n]    = sum_j down_e h[n][j]
  * gate and up are [F, K], down is [K, F] per expert, in q8_0 or q4_0 (one
  * format for gate and up, one for down); K % 32 == 0, F % 32 == 0, both at
- * most 2^20.  Activations are rounded to 22-bit block fixed point as in the
- * GEMVs.  x and y are fp32, bf16 or fp16 (QGEMV_F32 ...), y has x's type;
+ * most 2^20.  Activations (x of every type, and h) are rounded to block fixed
+ * point: a value moves by at most 2^-21.9 of the largest of its block of 32.
+ * x and y are fp32, bf16 or fp16 (QGEMV_F32 ...), y has x's type;
  * row n of x is at x + n * ldx elements, row n of y at y + n * ldy.
  *
  * Limits: E (shared experts included) <= 1024, choices per token (shared

@@ -41,22 +41,25 @@
 //
 // The arithmetic is the library's exact-integer scheme.  A block of 32
 // activations is rounded to integers X = rint(x FX / max |x|) and split into
-// signed byte digits X = p0 + 2^8 p1 (+ 2^16 p2); the integer dots of the
+// signed byte digits X = p0 + 2^8 p1 + 2^16 p2; the integer dots of the
 // block's quants with the digits are exact (mma.sync.m16n8k32.s8,
 // |S| <= 32 * 128 * 128 = 2^19), and each block is scaled once:
 // acc += (S0 + 2^8 S1 + 2^16 S2) (d max / FX).
 //
-//  * fp32 activations take three digits, FX = 0x7F7F7F (a step of max |x| 2^-23;
-//    the GEMVs' powers of two leave 2^-22 to 2^-21, and here two products
-//    follow one another: measured 7.5e-7 -> 2.9e-7 relative error of y);
-//  * bf16 and fp16 activations take two, FX = 0x7F7F: a step of max |x| 2^-15
-//    moves y by about 1e-5 of its size, a twentieth of fp16's own rounding of y
-//    (2^-12 on average) and a two-hundredth of bf16's, for x and for h.
+// FX = 0x7F7F7F for every type of x and for h: a step of max |x| 2^-23 (the
+// GEMVs' powers of two leave 2^-22 to 2^-21, and here two products follow one
+// another: measured 7.5e-7 -> 2.9e-7 relative error of y).  bf16 and fp16
+// activations do not get by with two digits, though two carry all their bits:
+// the step is the block's, 2^-15 of its largest value then, and an outlier
+// 1000 times its neighbours leaves them 1.5 % off, in full where a row's weight
+// on the outlier is 0.  (The third digit costs bf16 nothing at one token, 6 % at
+// 16 tokens over 64 experts in q8_0, 184 -> 195 us, and most where the
+// instructions count: 64 tokens, 128 experts in q4_0, 115 -> 158 us.)
 //
-// The 8 columns of an MMA are the digits of 4 tokens (two digits each) or 2
-// (three), so one MMA per block serves up to 4 or 2 tokens, and a lane's pair
-// of accumulators is one token's pair of digits, joined as integers
-// (|S0 + 2^8 S1| < 2^28) and converted once.
+// The 8 columns of an MMA are the digits of 2 tokens, so one MMA per block
+// serves up to 2, and a lane's pair of accumulators is one token's two low
+// digits, joined as integers (|S0 + 2^8 S1| < 2^28) and converted once, or its
+// high digit.
 // A block that holds a NaN or an infinity gets a NaN scale: y is NaN there.
 //
 // Weights are "expert tiles", laid out once: per expert, chunks of 64 rows (four
@@ -98,12 +101,12 @@ constexpr int DN_THREADS = 32 * (MOE_CW + 1);
 constexpr int MOE_DOWN_CL = 8;             // down: CTAs of a cluster, at most
 constexpr int MOE_GCOLS = 128;      // columns of a group (4 blocks)
 // digit bytes of a group: [digits][4 lanes][32]
-template <int DIG> __host__ __device__ constexpr int dig_bytes() { return DIG * 128; }
+constexpr int MOE_DIG = 3;
+constexpr int DIG_BYTES = MOE_DIG * 128;
 // tokens that share one MMA, and of one entry (one or two MMAs) at most: four
 // MMAs an entry do not fit the registers (they spilled 1 KB and cost all
 // calls 1.5x); an expert with more tokens streams its weights again, from L2
-template <int DIG> __host__ __device__ constexpr int tok_mma() { return DIG == 2 ? 4 : 2; }
-template <int DIG> __host__ __device__ constexpr int ent_tok() { return 2 * tok_mma<DIG>(); }
+constexpr int TOK_MMA = 2, MOE_ENT = 2 * TOK_MMA;
 
 // bytes of a group (16 rows x 128 columns): quants, then 64 fp16 scales
 template <int FMT> __host__ __device__ constexpr int grp_q() { return FMT == 8 ? 2048 : 1024; }
@@ -139,11 +142,9 @@ struct BlockScale {
   float s;      // FX / (max up); 0 for an all-zero or non-finite block (X = 0)
   float scale;  // max / FX; 0 for an all-zero block, NaN for a non-finite one
 };
-// 0x7F7F7F or 0x7F7F: every signed byte digit at most 127
-template <int DIG> __host__ __device__ constexpr int fx_max() { return DIG == 2 ? 0x7F7F : 0x7F7F7F; }
-template <int DIG>
+constexpr int FX_MAX = 0x7F7F7F;  // every signed byte digit at most 127
 __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
-  constexpr float FX = (float)fx_max<DIG>();
+  constexpr float FX = (float)FX_MAX;
   BlockScale b{1.0f, 0.0f, 0.0f};
   const float m = __uint_as_float(amax);
   if (amax >= 0x7F800000u) {
@@ -156,14 +157,12 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t amax) {
   }
   return b;
 }
-// X + 0x808080 (or 0x8080) of one value: byte p, with its top bit flipped, is
+// X + 0x808080 of one value: byte p, with its top bit flipped, is
 // digit p.  The clamp holds |X| <= FX also where the product rounds up, so the
 // biased value keeps to its digits.  A value of a non-finite block gives 0.
-template <int DIG>
 __device__ __forceinline__ uint32_t fixed_biased(float v, const BlockScale& b) {
-  constexpr int FX = fx_max<DIG>();
   const int X = b.s == 0.0f ? 0 : __float2int_rn(v * b.up * b.s);
-  return (uint32_t)(min(max(X, -FX), FX) + (DIG == 2 ? 0x8080 : 0x808080));
+  return (uint32_t)(min(max(X, -FX_MAX), FX_MAX) + 0x808080);
 }
 
 struct MoeArgs {
@@ -205,7 +204,6 @@ struct RouteArgs {
 // past K get zero digits and a zero scale.  Also the zero scales of h's blocks
 // past F (their digits are never read into a nonzero product, but a stale NaN
 // scale would be).
-template <int DIG>
 __device__ void prepare_x(const MoeArgs& a, int warp, int nwarps, int lane) {
   const int kg = groups_of(a.K), fg = groups_of(a.F), fb = a.F / QK;
   for (int i = warp; i < a.N * kg; i += nwarps) {
@@ -220,16 +218,16 @@ __device__ void prepare_x(const MoeArgs& a, int warp, int nwarps, int lane) {
     for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const BlockScale b = block_scale<DIG>(m);
+    const BlockScale b = block_scale(m);
     uint32_t f[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = fixed_biased<DIG>(v[j], b);
+    for (int j = 0; j < 4; ++j) f[j] = fixed_biased(v[j], b);
     // lane 8 blk + j holds elements 4j ... of block blk: B fragment register
     // j / 4 of MMA lane j % 4
     const int blk = lane >> 3, t = lane & 3, half = (lane >> 2) & 1;
-    uint8_t* dst = a.xdig + (int64_t)i * dig_bytes<DIG>() + t * 32 + blk * 8 + half * 4;
+    uint8_t* dst = a.xdig + (int64_t)i * DIG_BYTES + t * 32 + blk * 8 + half * 4;
 #pragma unroll
-    for (int p = 0; p < DIG; ++p) {
+    for (int p = 0; p < MOE_DIG; ++p) {
       const uint32_t w = ((f[0] >> (8 * p)) & 0xFFu) | (((f[1] >> (8 * p)) & 0xFFu) << 8) |
                          (((f[2] >> (8 * p)) & 0xFFu) << 16) | (((f[3] >> (8 * p)) & 0xFFu) << 24);
       *reinterpret_cast<uint32_t*>(dst + p * 128) = w ^ 0x80808080u;
@@ -391,8 +389,7 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route(MoeArgs a, RouteArg
     pdl_wait();
     const int w = (blockIdx.x - RT_CL * r.clusters) * RT_WARPS + warp;
     const int nw = (gridDim.x - RT_CL * r.clusters) * RT_WARPS;
-    if (a.xdt == 0) prepare_x<3>(a, w, nw, lane);
-    else prepare_x<2>(a, w, nw, lane);
+    prepare_x(a, w, nw, lane);
     return;
   }
   constexpr int CH = rt_chunk<TN>();
@@ -572,8 +569,7 @@ __global__ void __launch_bounds__(RT_THREADS, 2) k_moe_route_many(MoeArgs a, Rou
     pdl_wait();
     const int w = (blockIdx.x - RM_CL * r.clusters) * RT_WARPS + warp;
     const int nw = (gridDim.x - RM_CL * r.clusters) * RT_WARPS;
-    if (a.xdt == 0) prepare_x<3>(a, w, nw, lane);
-    else prepare_x<2>(a, w, nw, lane);
+    prepare_x(a, w, nw, lane);
     return;
   }
   cg::cluster_group cl = cg::this_cluster();
@@ -674,9 +670,8 @@ struct Table {
   __device__ __forceinline__ int run(int e) const {
     const uint32_t x = ent[e] & 1023u;
     const int c = __popc(mask[2 * x]) + __popc(mask[2 * x + 1]);
-    return (c + per_entry - 1) / per_entry;
+    return (c + MOE_ENT - 1) / MOE_ENT;
   }
-  int per_entry;
 };
 __host__ __device__ __forceinline__ size_t table_bytes(int E, int P, int max_ent) {
   return (size_t)(3 * E + max_ent + 3 * P) * 4;
@@ -687,7 +682,6 @@ __device__ __forceinline__ void clear_table(uint8_t* mem, const MoeArgs& a) {
   for (int i = threadIdx.x; i < 2 * a.E; i += blockDim.x) reinterpret_cast<uint32_t*>(mem)[i] = 0u;
   __syncthreads();
 }
-template <int MOE_ENT>
 __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   __shared__ uint32_t wsum[32];
   const int P = a.N * a.slots, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -721,8 +715,7 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
     }
     __syncthreads();
     t.nent = (int)wsum[0];
-    t.per_entry = MOE_ENT;
-    return t;
+      return t;
   }
   for (int p = tid; p < P; p += blockDim.x) {
     const uint32_t id = (uint32_t)a.ids[p];
@@ -780,7 +773,6 @@ __device__ Table build_table(uint8_t* mem, const MoeArgs& a) {
   }
   __syncthreads();
   t.nent = (int)(total >> 16);
-  t.per_entry = MOE_ENT;
   return t;
 }
 
@@ -939,31 +931,28 @@ struct Cols {
   const float* s;
   // row(i): the activation row of the i-th of `cnt` tokens; the columns of
   // absent tokens repeat the last one's
-  template <int DIG, typename Row>
+  template <typename Row>
   __device__ __forceinline__ void set(const uint8_t* digits, const float* scales, int groups, int cnt,
                                       int lane, Row row) {
     const int n = lane >> 2, t = lane & 3;
-    // three digits: column 3 (and 7) is idle and reads digit 2 again; its
-    // accumulator is dropped
-    const int tok = DIG == 2 ? n >> 1 : n >> 2, d = DIG == 2 ? n & 1 : min(n & 3, 2);
-    dig = digits + row(min(tok, cnt - 1)) * groups * dig_bytes<DIG>() + d * 128 + t * 32;
-    s = scales + row(min(DIG == 2 ? t : t >> 1, cnt - 1)) * groups * 4;
+    // column 3 (and 7) is idle and reads digit 2 again; its accumulator is dropped
+    const int tok = n >> 2, d = min(n & 3, 2);
+    dig = digits + row(min(tok, cnt - 1)) * groups * DIG_BYTES + d * 128 + t * 32;
+    s = scales + row(min(t >> 1, cnt - 1)) * groups * 4;
   }
   // group j from here
-  template <int DIG>
   __device__ __forceinline__ void load(Digits& f, int j) const {
-    f.b[0] = ldg128(dig + j * dig_bytes<DIG>());
-    f.b[1] = ldg128(dig + j * dig_bytes<DIG>() + 16);
+    f.b[0] = ldg128(dig + j * DIG_BYTES);
+    f.b[1] = ldg128(dig + j * DIG_BYTES + 16);
     f.s = ldg128(s + j * 4);
   }
-  template <int DIG>
   __device__ __forceinline__ Cols at(int grp) const {
-    return Cols{dig + (int64_t)grp * dig_bytes<DIG>(), s + (int64_t)grp * 4};
+    return Cols{dig + (int64_t)grp * DIG_BYTES, s + (int64_t)grp * 4};
   }
 };
 
-// acc[0], acc[1]: rows g and g + 8 of the lane's token (three digits: the even
-// lane holds the two low digits' sum, the odd one the high digit's); blocks
+// acc[0], acc[1]: rows g and g + 8 of the lane's token (the even lane holds
+// the two low digits' sum, the odd one the high digit's); blocks
 // 2 p and 2 p + 1.  w: the second column's weight (256, or 0 in the odd lane).
 template <int FMT>
 __device__ __forceinline__ void product(float* acc, const Quants<FMT>& q, const Digits& f, int p, int w) {
@@ -982,9 +971,9 @@ __device__ __forceinline__ void product(float* acc, const Quants<FMT>& q, const 
 // sums.  Four sets of digits fit the registers: two groups of one or two MMAs
 // of tokens (q8_0), four groups of one MMA (q4_0); a q4_0 slab with two MMAs
 // keeps two groups and reads on inside the slab.
-template <int FMT, int DIG>
+template <int FMT>
 struct Work {
-  static constexpr int T = tok_mma<DIG>(), SG = slab_groups<FMT>();
+  static constexpr int T = TOK_MMA, SG = slab_groups<FMT>();
   // the slab ahead: its tokens' digits (of its first group), groups and width
   struct Ahead {
     Cols c0, c1;
@@ -1000,13 +989,13 @@ struct Work {
   __device__ __forceinline__ void entry(const uint8_t* digits, const float* scales, int groups, int cnt,
                                         int lane, Row row) {
     etwo = cnt > T;
-    e0.template set<DIG>(digits, scales, groups, cnt, lane, row);
-    if (etwo) e1.template set<DIG>(digits, scales, groups, cnt - T, lane, [&](int i) { return row(T + i); });
+    e0.set(digits, scales, groups, cnt, lane, row);
+    if (etwo) e1.set(digits, scales, groups, cnt - T, lane, [&](int i) { return row(T + i); });
   }
   __device__ __forceinline__ Ahead ahead(int grp, int m) const {
     Ahead a;
-    a.c0 = e0.template at<DIG>(grp);
-    a.c1 = e1.template at<DIG>(grp);
+    a.c0 = e0.at(grp);
+    a.c1 = e1.at(grp);
     a.m = m;
     a.two = etwo;
     return a;
@@ -1017,8 +1006,8 @@ struct Work {
   }
   template <bool TWO>
   __device__ __forceinline__ void load(const Ahead& a, int j) {
-    a.c0.template load<DIG>(f[slot(TWO, j, 0)], j);
-    if (TWO) a.c1.template load<DIG>(f[slot(TWO, j, 1)], j);
+    a.c0.load(f[slot(TWO, j, 0)], j);
+    if (TWO) a.c1.load(f[slot(TWO, j, 1)], j);
   }
   // what a slab starts with
   __device__ __forceinline__ void begin(const Ahead& a) {
@@ -1038,7 +1027,7 @@ struct Work {
   }
   template <bool TWO>
   __device__ __forceinline__ void groups(uint32_t st, const Ahead& now, const Ahead& next, int lane) {
-    const int w = DIG == 3 && (lane & 1) ? 0 : 256;
+    const int w = lane & 1 ? 0 : 256;
     const int nm = whole(TWO) && next.two == TWO ? next.m : 0;
 #pragma unroll
     for (int j = 0; j < SG; ++j) {
@@ -1079,13 +1068,13 @@ struct Work {
     const int t = lane & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      acc[i] *= DIG == 3 && (t & 1) ? 65536.0f * Q : Q;
-      if (DIG == 3) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);  // the high digit's lane
+      acc[i] *= t & 1 ? 65536.0f * Q : Q;
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);  // the high digit's lane
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int i = c * T + (DIG == 2 ? t : t >> 1);
-      if ((DIG == 2 || !(t & 1)) && i < cnt) put(i, acc[2 * c], acc[2 * c + 1]);
+      const int i = c * T + (t >> 1);
+      if (!(t & 1) && i < cnt) put(i, acc[2 * c], acc[2 * c + 1]);
     }
   }
 };
@@ -1093,22 +1082,22 @@ struct Work {
 // ------------------------------------------------------------- gate and up
 // The compute warps leave a unit's sums (per split) in one of two buffers and
 // go on; three further warps add the splits, form h and round it.
-template <int DIG> struct UpPart {
-  float v[2][MOE_KS][ent_tok<DIG>()][72];  // [buffer][split][token][32 gate, 32 up, padding]
+struct UpPart {
+  float v[2][MOE_KS][MOE_ENT][72];  // [buffer][split][token][32 gate, 32 up, padding]
 };
-template <int FMT, int DIG>
+template <int FMT>
 __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
   extern __shared__ __align__(128) uint8_t up_smem[];
   __shared__ __align__(8) Pipe pipe;
   constexpr int SG = slab_groups<FMT>(), GB = grp_bytes<FMT>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) pipe.init();
-  uint8_t* const table = up_smem + ring_bytes<FMT>() + sizeof(UpPart<DIG>);
+  uint8_t* const table = up_smem + ring_bytes<FMT>() + sizeof(UpPart);
   clear_table(table, a);
   pdl_wait();
   pdl_trigger();
-  UpPart<DIG>& part = *reinterpret_cast<UpPart<DIG>*>(up_smem + ring_bytes<FMT>());
-  const Table tb = build_table<ent_tok<DIG>()>(table, a);
+  UpPart& part = *reinterpret_cast<UpPart*>(up_smem + ring_bytes<FMT>());
+  const Table tb = build_table(table, a);
   const int fc = a.F / 32, kg = groups_of(a.K), fg = groups_of(a.F), ns = (kg + SG - 1) / SG;
   const int units = tb.nent * fc, G = gridDim.x;
   // unit u: entry u / fc, chunk u % fc, stepped without divisions
@@ -1153,7 +1142,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
   } else if (warp < MOE_CW) {
     // ------------------------------------------------------------- compute
     const int rt = warp % MOE_RT, kq = warp / MOE_RT;
-    Work<FMT, DIG> w;
+    Work<FMT> w;
     w.clear();
     // the unit whose sums are under way (number j here, entry en) and the slab
     // ahead: slab i of the CTA is split i % 3's, counted on through the units
@@ -1168,7 +1157,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       w.entry(a.xdig, a.xs, kg, (en >> 22) & 15, lane, [&](int i) { return (int64_t)(tb.sorted[at + i] >> 16); });
     };
     auto peek = [&]() {  // the slab ahead, over units that have none for this split
-      typename Work<FMT, DIG>::Ahead x;
+      typename Work<FMT>::Ahead x;
       bool moved = false;
       while (al >= ns) {
         step();
@@ -1180,7 +1169,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       if (moved) take();
       return w.ahead(al * SG, min(SG, kg - al * SG));
     };
-    typename Work<FMT, DIG>::Ahead now;
+    typename Work<FMT>::Ahead now;
     if (pos.u < units) {
       take();
       now = peek();
@@ -1237,12 +1226,12 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
         const int64_t row = tb.sorted[at + i] & 0xFFFFu;
         const float v = gate / (1.0f + expf(-gate)) * up * tb.w[row];
         const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7FFFFFFFu);
-        const BlockScale bs = block_scale<DIG>(m);
-        const uint32_t f = fixed_biased<DIG>(v, bs) ^ 0x808080u;
-        uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * dig_bytes<DIG>() + ((lane >> 2) & 3) * 32 +
+        const BlockScale bs = block_scale(m);
+        const uint32_t f = fixed_biased(v, bs) ^ 0x808080u;
+        uint8_t* dst = a.hdig + (row * fg + (hb >> 2)) * DIG_BYTES + ((lane >> 2) & 3) * 32 +
                        (hb & 3) * 8 + (lane >> 4) * 4 + (lane & 3);
 #pragma unroll
-        for (int p = 0; p < DIG; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
+        for (int p = 0; p < MOE_DIG; ++p) dst[p * 128] = (uint8_t)(f >> (8 * p));
         if (lane == 0) a.hs[row * fg * 4 + hb] = bs.scale;
       }
       __syncwarp();
@@ -1255,7 +1244,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
 // A cluster's CTAs have the same 64 rows of y and share out the entries' slabs,
 // entry after entry, cut anywhere; the three splits of a CTA add into a copy of
 // the 64 rows each.
-template <int FMT, int DIG>
+template <int FMT>
 __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) {
   extern __shared__ __align__(128) uint8_t dn_smem[];
   __shared__ __align__(8) Pipe pipe;
@@ -1275,7 +1264,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
   // (the producer's for empty stages) counts k_moe_up's time.
   pdl_wait();
   pdl_trigger();
-  const Table tb = build_table<ent_tok<DIG>()>(table, a);
+  const Table tb = build_table(table, a);
   const int fg = groups_of(a.F), fs = (fg + SG - 1) / SG, chunks = (a.K + R - 1) / R;
   const int64_t total = (int64_t)tb.nent * fs;
   const int q0 = (int)(total * rank / cs), q1 = (int)(total * (rank + 1) / cs);
@@ -1297,7 +1286,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
   } else {
     const int rt = warp % MOE_RT, kq = warp / MOE_RT;
     float* yp = ypart + kq * yn + rt * 16 + (lane >> 2);
-    Work<FMT, DIG> w;
+    Work<FMT> w;
     w.clear();
     // slab q of entry e (`en`: its tokens), and the slab ahead (al of entry ae)
     int q = q0 + kq, ae = q / fs, al = q - ae * fs;
@@ -1306,7 +1295,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
       const int at = (en >> 10) & 0xFFF;
       w.entry(a.hdig, a.hs, fg, (en >> 22) & 15, lane, [&](int i) { return (int64_t)(tb.sorted[at + i] & 0xFFFFu); });
     };
-    typename Work<FMT, DIG>::Ahead now;
+    typename Work<FMT>::Ahead now;
     uint32_t en = 0;
     if (q < q1) {
       en = tb.ent[ae];
@@ -1315,7 +1304,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
       w.begin(now);
     }
     while (q < q1) {
-      typename Work<FMT, DIG>::Ahead next;
+      typename Work<FMT>::Ahead next;
       uint32_t nen = en;
       q += MOE_KS;
       if (q < q1) {
@@ -1443,11 +1432,11 @@ WsMap ws_map(int64_t N, int slots, int64_t K, int64_t F) {
   m.weights = o;
   o += up(n * slots * 4);
   m.xdig = o;
-  o += up(n * kg * dig_bytes<3>());
+  o += up(n * kg * DIG_BYTES);
   m.xs = o;
   o += up(n * kg * 16);
   m.hdig = o;
-  o += up(n * slots * fg * dig_bytes<3>());
+  o += up(n * slots * fg * DIG_BYTES);
   m.hs = o;
   o += up(n * slots * fg * 16);
   m.bytes = o;
@@ -1534,27 +1523,27 @@ int launch_route(const MoeArgs& a, RouteArgs r, bool route, bool prep, const Dev
   return launch("k_moe_route", k_moe_route_many, dim3(RM_CL * r.clusters + pre), RT_THREADS, smem, RM_CL, st, a, r);
 }
 
-template <int FMT, int DIG>
+template <int FMT>
 size_t up_smem(int E, int P, int max_ent) {
-  return (size_t)ring_bytes<FMT>() + sizeof(UpPart<DIG>) + table_bytes(E, P, max_ent);
+  return (size_t)ring_bytes<FMT>() + sizeof(UpPart) + table_bytes(E, P, max_ent);
 }
 template <int FMT>
 size_t dn_smem(int E, int P, int max_ent, int N) {
   return (size_t)ring_bytes<FMT>() + (size_t)MOE_KS * N * 16 * MOE_RT * 4 + table_bytes(E, P, max_ent);
 }
 
-template <int FMT, int DIG>
+template <int FMT>
 int launch_up(const MoeArgs& a, const DeviceInfo& dev, cudaStream_t st) {
-  if (int rc = allow_max_smem((const void*)k_moe_up<FMT, DIG>, dev)) return rc;
-  const size_t smem = up_smem<FMT, DIG>(a.E, a.N * a.slots, a.max_ent);
+  if (int rc = allow_max_smem((const void*)k_moe_up<FMT>, dev)) return rc;
+  const size_t smem = up_smem<FMT>(a.E, a.N * a.slots, a.max_ent);
   const int64_t units = (int64_t)a.max_ent * (a.F / 32);
   const dim3 grid((unsigned)std::min<int64_t>(units, dev.sms));
-  return launch("k_moe_up", k_moe_up<FMT, DIG>, grid, UP_THREADS, smem, 0, st, a);
+  return launch("k_moe_up", k_moe_up<FMT>, grid, UP_THREADS, smem, 0, st, a);
 }
 
-template <int FMT, int DIG>
+template <int FMT>
 int launch_down(const MoeArgs& a, int ydt, const DeviceInfo& dev, cudaStream_t st) {
-  if (int rc = allow_max_smem((const void*)k_moe_down<FMT, DIG>, dev)) return rc;
+  if (int rc = allow_max_smem((const void*)k_moe_down<FMT>, dev)) return rc;
   const size_t smem = dn_smem<FMT>(a.E, a.N * a.slots, a.max_ent, a.N);
   const int chunks = (a.K + 16 * MOE_RT - 1) / (16 * MOE_RT);
   // CTAs that share 64 rows: as many as leaves every cluster resident at once
@@ -1563,11 +1552,11 @@ int launch_down(const MoeArgs& a, int ydt, const DeviceInfo& dev, cudaStream_t s
   int cs = MOE_DOWN_CL;
   while (cs > 1) {
     int most = 0;
-    if (int rc = active_clusters((const void*)k_moe_down<FMT, DIG>, dev, DN_THREADS, smem, cs, &most)) return rc;
+    if (int rc = active_clusters((const void*)k_moe_down<FMT>, dev, DN_THREADS, smem, cs, &most)) return rc;
     if (chunks <= most) break;
     --cs;
   }
-  return launch("k_moe_down", k_moe_down<FMT, DIG>, dim3(chunks * cs), DN_THREADS, smem, cs, st, a, ydt);
+  return launch("k_moe_down", k_moe_down<FMT>, dim3(chunks * cs), DN_THREADS, smem, cs, st, a, ydt);
 }
 
 }  // namespace
@@ -1637,10 +1626,9 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
   const int64_t xb = xdt == 0 ? 4 : 2;
   // tokens of a pass: 64, or fewer where many experts or choices leave too
   // little shared memory for the entries (1024 experts with 32 choices: 32)
-  const int et = xdt == 0 ? ent_tok<3>() : ent_tok<2>();
   int nt = MOE_NT;
-  auto ents = [&](int n) { return std::min(m.E, n * slots) + n * slots / et; };
-  while (nt > 1 && std::max(up_smem<4, 2>(m.E, nt * slots, ents(nt)),
+  auto ents = [&](int n) { return std::min(m.E, n * slots) + n * slots / MOE_ENT; };
+  while (nt > 1 && std::max(up_smem<4>(m.E, nt * slots, ents(nt)),
                             dn_smem<4>(m.E, nt * slots, ents(nt), nt)) + 1024 > (size_t)dev.smem_optin)
     nt /= 2;
   for (int64_t n0 = 0; n0 < N; n0 += nt) {
@@ -1681,13 +1669,8 @@ int moe_experts(const MoeExperts& m, const MoeRoute* route, const void* x, int x
       r.weights = reinterpret_cast<float*>(w + wm.weights);
     }
     if (int rc = launch_route(a, r, route != nullptr, true, dev, st)) return rc;
-    int rc;
-    if (xdt == 0) rc = m.fmt == 8 ? launch_up<8, 3>(a, dev, st) : launch_up<4, 3>(a, dev, st);
-    else rc = m.fmt == 8 ? launch_up<8, 2>(a, dev, st) : launch_up<4, 2>(a, dev, st);
-    if (rc) return rc;
-    if (xdt == 0) rc = m.fmt_down == 8 ? launch_down<8, 3>(a, xdt, dev, st) : launch_down<4, 3>(a, xdt, dev, st);
-    else rc = m.fmt_down == 8 ? launch_down<8, 2>(a, xdt, dev, st) : launch_down<4, 2>(a, xdt, dev, st);
-    if (rc) return rc;
+    if (int rc = m.fmt == 8 ? launch_up<8>(a, dev, st) : launch_up<4>(a, dev, st)) return rc;
+    if (int rc = m.fmt_down == 8 ? launch_down<8>(a, xdt, dev, st) : launch_down<4>(a, xdt, dev, st)) return rc;
   }
   return OK;
 }

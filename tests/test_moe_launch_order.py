@@ -27,7 +27,7 @@ def body(kernel):
 
 
 @pytest.mark.parametrize("kernel", ["k_moe_up", "k_moe_down"])
-@pytest.mark.parametrize("use", ["build_table<", ".put(", "mbar_wait(", ".entry(", "a.ids", "a.weights", "a.hdig", "a.xdig"])
+@pytest.mark.parametrize("use", ["build_table", ".put(", "mbar_wait(", ".entry(", "a.ids", "a.weights", "a.hdig", "a.xdig"])
 def test_nothing_global_and_no_bounded_wait_before_the_dependency_wait(kernel, use):
     text = body(kernel)
     assert text.count("pdl_wait();") == 1
