@@ -6,6 +6,7 @@ reads and no temporary objects."""
 from __future__ import annotations
 
 import functools
+import threading
 
 import torch
 
@@ -70,8 +71,17 @@ def stream_of(stream, device) -> int:
     return _raw_stream(device.index) if stream is None else stream
 
 
-# one per (device, stream), grown on demand: calls on one stream are ordered
-_WS: dict = {}
+class Workspaces(threading.local):
+    """Buffers by (device, stream), grown on demand, of one host thread.  Calls
+    of a thread on a stream are ordered and share a buffer; a call is several
+    launches that pass data through it, and another thread's launches on the
+    same stream may come between them (the C call runs without the GIL)."""
+
+    def __init__(self):
+        self.buffers: dict = {}
+
+
+_WS = Workspaces()
 
 
 def workspace(device, nbytes: int, stream):
@@ -85,8 +95,9 @@ def workspace(device, nbytes: int, stream):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         return ws, ws.data_ptr(), nbytes
     key = (device.index, _raw_stream(device.index))
-    ws = _WS.get(key)
+    buffers = _WS.buffers
+    ws = buffers.get(key)
     if ws is None or ws[2] < nbytes:
         t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws = _WS[key] = (t, t.data_ptr(), nbytes)
+        ws = buffers[key] = (t, t.data_ptr(), nbytes)
     return ws

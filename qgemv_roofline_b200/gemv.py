@@ -16,6 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from ._tensors import Workspaces
 from .qformats import BLOCK_BYTES, QK
 
 _SOA_FN = {"q8_0": "qgemv_q8_0_soa", "q4_0": "qgemv_q4_0_soa"}
@@ -67,9 +68,8 @@ def _xy(x: torch.Tensor, M: int, K: int, y: torch.Tensor | None, device):
     return X, Y, y, N, ldx, ldy
 
 
-# Workspaces of the batched calls, one per (device, torch stream), grown on
-# demand: calls on one stream are ordered, so they may share it.
-_WS: dict = {}
+# Workspaces of the batched calls, one per (host thread, device, torch stream).
+_WS = Workspaces()
 
 
 def _workspace(device, nbytes: int, stream) -> torch.Tensor:
@@ -82,10 +82,11 @@ def _workspace(device, nbytes: int, stream) -> torch.Tensor:
     if stream is not None or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, cur.stream_id, cur.cuda_stream)
-    ws = _WS.get(key)
+    buffers = _WS.buffers
+    ws = buffers.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _WS[key] = ws
+        buffers[key] = ws
     return ws
 
 
