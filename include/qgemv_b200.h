@@ -167,7 +167,9 @@ QGEMV_API int qgemv_soa_ws(int format, const void* q, const void* d, const float
                            int64_t M, int64_t K, int32_t ncols, int64_t ldx, int64_t ldy,
                            void* workspace, size_t workspace_bytes, void* stream);
 
-/* Frees the per-stream workspaces (synchronises their devices). */
+/* Frees the per-stream workspaces (synchronises their devices).  Calls of
+ * several threads on one stream take turns with its workspace, a call at a
+ * time; a workspace that the caller brings is the caller's to keep apart. */
 QGEMV_API int qgemv_release_workspaces(void);
 
 /* qgemv_soa_ws with the workspace taken from a 2 MiB array compiled into the

@@ -14,6 +14,7 @@
 #include <mutex>
 #include <map>
 #include <set>
+#include <thread>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -218,6 +219,7 @@ int gemv_entry(int fmt, bool aos, const void* q, const void* d, const float* x, 
   c.ldx = ldx;
   c.ldy = ldy;
   c.no_tc = !allow_tc;
+  WorkspaceHold hold;
   if (!aos) {
     // the tensor-core batch kernels need a workspace: the caller's, or one
     // cached for this stream
@@ -231,7 +233,7 @@ int gemv_entry(int fmt, bool aos, const void* q, const void* d, const float* x, 
           return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need,
                            ws_bytes);
         if (misaligned(ws, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-      } else if (int rc = stream_workspace(st, need, &ws)) {
+      } else if (int rc = stream_workspace(st, need, &ws, hold)) {
         return rc;
       } else {
         ws_bytes = need;
@@ -243,20 +245,34 @@ int gemv_entry(int fmt, bool aos, const void* q, const void* d, const float* x, 
   return aos ? gemv_aos(fmt, c, st) : gemv_soa(fmt, c, st);
 }
 
-// Per-(device, stream) workspaces of the plain entry points.
+// Per-(device, stream) workspaces of the plain entry points.  g_ws_mu guards
+// the map, whose entries stay; an entry's own mutex its buffer, and is never
+// held while g_ws_mu is asked for.  The per-thread default stream has one
+// handle for every thread's stream, hence the thread.
+struct StreamWorkspace {
+  std::mutex mu;
+  void* p = nullptr;
+  size_t bytes = 0;
+};
 std::mutex g_ws_mu;
-std::map<std::pair<int, cudaStream_t>, std::pair<void*, size_t>> g_ws;
+std::map<std::tuple<int, cudaStream_t, std::thread::id>, StreamWorkspace> g_ws;
 
 }  // namespace
 
-int stream_workspace(cudaStream_t st, size_t bytes, void** out) {
+int stream_workspace(cudaStream_t st, size_t bytes, void** out, WorkspaceHold& hold) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_error(ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
-  std::lock_guard<std::mutex> lk(g_ws_mu);
-  auto& slot = g_ws[std::make_pair(dev, st)];
-  if (slot.first && slot.second >= bytes) {
-    *out = slot.first;
+  const std::thread::id thread = st == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id();
+  StreamWorkspace* slot;
+  {
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    slot = &g_ws[std::make_tuple(dev, st, thread)];
+  }
+  WorkspaceHold own(slot->mu);
+  if (slot->p && slot->bytes >= bytes) {
+    *out = slot->p;
+    hold = std::move(own);
     return OK;
   }
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
@@ -267,19 +283,22 @@ int stream_workspace(cudaStream_t st, size_t bytes, void** out) {
                      "allocated during stream capture: make one uncaptured call of this shape "
                      "on the stream first, or pass a workspace (qgemv_soa_ws)",
                      bytes);
-  const size_t grow = std::max(bytes, slot.second * 2);
-  if (slot.first) {
+  const size_t grow = std::max(bytes, slot->bytes * 2);
+  if (slot->p) {
     // the old buffer may still be read by work queued on this stream
-    if ((e = cudaStreamSynchronize(st)) != cudaSuccess || (e = cudaFree(slot.first)) != cudaSuccess)
+    if ((e = cudaStreamSynchronize(st)) != cudaSuccess || (e = cudaFree(slot->p)) != cudaSuccess)
       return set_error(ERR_CUDA, "releasing the stream workspace: %s", cudaGetErrorString(e));
-    slot = std::make_pair(nullptr, (size_t)0);
+    slot->p = nullptr;
+    slot->bytes = 0;
   }
   void* p = nullptr;
   if ((e = cudaMalloc(&p, grow)) != cudaSuccess)
     return set_error(ERR_CUDA, "allocating a %zu-byte stream workspace: %s", grow,
                      cudaGetErrorString(e));
-  slot = std::make_pair(p, grow);
+  slot->p = p;
+  slot->bytes = grow;
   *out = p;
+  hold = std::move(own);
   return OK;
 }
 
@@ -287,17 +306,19 @@ int release_workspaces() {
   std::lock_guard<std::mutex> lk(g_ws_mu);
   int rc = OK;
   for (auto& kv : g_ws) {
-    if (!kv.second.first) continue;
+    WorkspaceHold own(kv.second.mu);  // a call under way has enqueued its launches
+    if (!kv.second.p) continue;
     int cur = 0;
     cudaGetDevice(&cur);
-    cudaSetDevice(kv.first.first);
+    cudaSetDevice(std::get<0>(kv.first));
     cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaFree(kv.second.first);
+    if (e == cudaSuccess) e = cudaFree(kv.second.p);
+    kv.second.p = nullptr;
+    kv.second.bytes = 0;
     cudaSetDevice(cur);
     if (e != cudaSuccess && rc == OK)
       rc = set_error(ERR_CUDA, "releasing a stream workspace: %s", cudaGetErrorString(e));
   }
-  g_ws.clear();
   return rc;
 }
 
@@ -685,12 +706,13 @@ QGEMV_API int qgemv_tiled_gemv(int format, const void* tiled, int64_t M, int64_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (K == 0) return fill_zero_rows(y, M, ncols, ldy, st);
   const size_t need = mma_workspace_bytes(K, ncols);
+  WorkspaceHold hold;
   if (workspace) {
     if (workspace_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need,
                        workspace_bytes);
     if (misaligned(workspace, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = stream_workspace(st, need, &workspace)) {
+  } else if (int rc = stream_workspace(st, need, &workspace, hold)) {
     return rc;
   } else {
     workspace_bytes = need;
@@ -762,12 +784,13 @@ QGEMV_API int qgemv_tc_gemv(int format, const void* tiles, int64_t M, int64_t K,
   DeviceInfo dev;
   if (int rc = current_device_info(dev)) return rc;
   const size_t need = tc_workspace_bytes(M, K, dev.sms);
+  WorkspaceHold hold;
   if (workspace) {
     if (workspace_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need,
                        workspace_bytes);
     if (misaligned(workspace, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = stream_workspace(st, need, &workspace)) {
+  } else if (int rc = stream_workspace(st, need, &workspace, hold)) {
     return rc;
   } else {
     workspace_bytes = need;
@@ -912,7 +935,7 @@ namespace {
 // The stream's workspace for a call that brought none.  Refused under capture:
 // a graph would keep the buffer's address, which a later, larger call on the
 // stream frees, and graphs captured on one stream would share it.
-int own_workspace(cudaStream_t st, size_t need, void** ws) {
+int own_workspace(cudaStream_t st, size_t need, void** ws, WorkspaceHold& hold) {
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   const cudaError_t e = cudaStreamIsCapturing(st, &cs);
   if (e != cudaSuccess) {
@@ -921,7 +944,7 @@ int own_workspace(cudaStream_t st, size_t need, void** ws) {
   }
   if (cs != cudaStreamCaptureStatusNone)
     return set_error(ERR_UNSUPPORTED, "a captured call needs a workspace of its own (%zu bytes)", need);
-  return stream_workspace(st, need, ws);
+  return stream_workspace(st, need, ws, hold);
 }
 
 int check_moe_x(const void* x, int dtype, int64_t ldx, int64_t N, int64_t K) {
@@ -999,11 +1022,12 @@ int moe_entry(const qgemv_expert_set* m, const qgemv_moe_router* router, const v
     return set_error(ERR_SHAPE, "ldy=%lld < hidden=%lld", (long long)ldy, (long long)m->hidden);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t need = moe_workspace_bytes(N, slots, m->hidden, m->ffn);
+  WorkspaceHold hold;
   if (ws) {
     if (ws_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, ws_bytes);
     if (misaligned(ws, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = own_workspace(st, need, &ws)) {
+  } else if (int rc = own_workspace(st, need, &ws, hold)) {
     return rc;
   }
   MoeExperts e;
@@ -1151,11 +1175,12 @@ QGEMV_API int qgemv_int8_linear(const void* x, int dtype, int64_t ldx, const voi
   if (ldy < (N > 1 ? M : 0)) return set_error(ERR_SHAPE, "ldy=%lld < M=%lld", (long long)ldy, (long long)M);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t need = qgemv_int8_linear_workspace_bytes(N, K);
+  WorkspaceHold hold;
   if (workspace) {
     if (workspace_bytes < need)
       return set_error(ERR_ARG, "this call needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
     if (misaligned(workspace, 16)) return set_error(ERR_ALIGN, "workspace must be 16-byte aligned");
-  } else if (int rc = own_workspace(st, need, &workspace)) {
+  } else if (int rc = own_workspace(st, need, &workspace, hold)) {
     return rc;
   }
   float* xs = static_cast<float*>(workspace);

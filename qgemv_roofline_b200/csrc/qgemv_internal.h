@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace qg {
 
 // Shared-memory budget for the staged activation tile of the GEMV kernels.
@@ -146,8 +148,12 @@ int encode_tensor_2d(CUtensorMap* map, bool u16, const void* base, uint64_t inne
 int set_tc_spin_limit(long long cycles);
 int read_tc_error(int clear, cudaStream_t st, int* out);
 // Workspace cached per (device, stream) for callers that pass none; grows on
-// demand (cudaMalloc, outside stream capture only).
-int stream_workspace(cudaStream_t st, size_t bytes, void** out);
+// demand (cudaMalloc, outside stream capture only).  `hold` keeps it for the
+// caller until its launches are enqueued: another thread's call on the stream
+// waits for that, so that its launches do not come between them (they would
+// overwrite what this call's launches pass on) and do not free the buffer.
+using WorkspaceHold = std::unique_lock<std::mutex>;
+int stream_workspace(cudaStream_t st, size_t bytes, void** out, WorkspaceHold& hold);
 // The fixed per-device workspace of qgemv_soa_static_ws (static_ws.cu).
 constexpr size_t kStaticWsBytes = (size_t)2 << 20;
 int static_workspace(void** out, size_t* bytes);

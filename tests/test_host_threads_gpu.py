@@ -64,3 +64,30 @@ def test_threads_on_the_default_stream(op):
     torch.cuda.synchronize()
     for ys, w in zip(got, want):
         assert len(ys) == 300 and all(torch.equal(y, w) for y in ys)
+
+
+@pytest.mark.parametrize("op", [0, 1])
+def test_threads_on_one_raw_stream(op):
+    """The library's own workspace of a stream, which grows while another thread's calls use it."""
+    g = torch.Generator(DEV).manual_seed(7)
+    K = 256
+    w = [torch.randn(6, *s, device=DEV, generator=g) * s[1] ** -0.5 for s in ((128, K), (128, K), (K, 128))]
+    experts = qg.QuantizedExperts.from_float(*w, "q8_0")
+    router = torch.randn(6, K, device=DEV, generator=g) * 0.2
+    wq, ws = qg.quantize_int8(torch.randn(K, K, device=DEV, generator=g))
+    call = [lambda x, **kw: qg.moe_layer(x, router, experts, 2, **kw), lambda x, **kw: qg.int8_linear(x, wq, ws, **kw)][op]
+    sizes = (1, 6, 40, 64)
+    xs = [torch.randn(n, K, device=DEV, generator=g) for n in sizes]
+    want = [call(x) for x in xs]
+    ys = [[torch.zeros_like(x) for _ in range(100)] for x in xs]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def work(i):
+        for y in ys[i]:
+            call(xs[i], y=y, stream=stream.cuda_stream)
+
+    in_threads(work, len(xs))
+    stream.synchronize()
+    for got, w in zip(ys, want):
+        assert all(torch.equal(y, w) for y in got)
