@@ -6,6 +6,7 @@ reads and no temporary objects."""
 from __future__ import annotations
 
 import functools
+import inspect
 import threading
 
 import torch
@@ -19,16 +20,22 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 
 
 def on_device_of_x(fn):
-    """Runs ``fn(x, ...)`` with the device of ``x`` current."""
+    """Runs ``fn(x, ...)`` with the device of its first argument current, which
+    may be given by its name, too."""
+    name = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def wrapper(x, *args, **kwargs):
+    def wrapper(*args, **kwargs):
+        if not args and name not in kwargs:
+            return fn(**kwargs)  # Python's own error
+        x = args[0] if args else kwargs[name]
         index = x.get_device() if isinstance(x, torch.Tensor) else -1
         if index < 0:
-            raise ValueError("x must be a CUDA tensor")
+            raise ValueError(f"{name} must be a CUDA tensor")
         if index == _current_device():
-            return fn(x, *args, **kwargs)
+            return fn(*args, **kwargs)
         with torch.cuda.device(index):
-            return fn(x, *args, **kwargs)
+            return fn(*args, **kwargs)
     return wrapper
 
 
