@@ -19,10 +19,41 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def stream_argument(fn):
+    """A function that finds the ``stream`` argument of a call of ``fn``."""
+    params = list(inspect.signature(fn).parameters.values())
+    at = next(i for i, p in enumerate(params) if p.name == "stream")
+    at = at if params[at].kind is not inspect.Parameter.KEYWORD_ONLY else len(params)
+
+    def find(args, kwargs):
+        return args[at] if len(args) > at else kwargs.get("stream")
+    return find
+
+
+def run_on(stream: int, index: int, fn, args, kwargs):
+    """``fn(*args, **kwargs)``, whose kernels go to the raw stream ``stream`` of
+    device ``index``, with that stream current: what it copies and allocates on
+    the way (an x with other strides, a workspace, y) is then ordered with the
+    kernels and goes back to the stream's own memory.  What it returns may be
+    used on the caller's stream, so its memory waits for that one too."""
+    caller = torch.cuda.current_stream(index)
+    if stream == caller.cuda_stream:
+        with torch.cuda.device(index):
+            return fn(*args, **kwargs)
+    # 0 and 1 are the handles of the legacy default stream
+    other = torch.cuda.default_stream(index) if stream in (0, 1) else torch.cuda.ExternalStream(stream, device=index)
+    with torch.cuda.stream(other):  # and its device
+        out = fn(*args, **kwargs)
+    for t in out if isinstance(out, tuple) else (out,):
+        t.record_stream(caller)
+    return out
+
+
 def on_device_of_x(fn):
     """Runs ``fn(x, ...)`` with the device of its first argument current, which
-    may be given by its name, too."""
+    may be given by its name, too, and the raw ``stream`` where one is given."""
     name = next(iter(inspect.signature(fn).parameters))
+    stream_of_call = stream_argument(fn)
 
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
@@ -32,6 +63,9 @@ def on_device_of_x(fn):
         index = x.get_device() if isinstance(x, torch.Tensor) else -1
         if index < 0:
             raise ValueError(f"{name} must be a CUDA tensor")
+        stream = stream_of_call(args, kwargs)
+        if stream is not None:
+            return run_on(stream, index, fn, args, kwargs)
         if index == _current_device():
             return fn(*args, **kwargs)
         with torch.cuda.device(index):
@@ -93,9 +127,8 @@ _WS = Workspaces()
 
 def workspace(device, nbytes: int, stream):
     """(tensor, pointer, bytes) of a call's workspace.  Under capture a buffer
-    of its own, from the graph's memory; for a raw stream handle none (the
-    library's own buffer of that stream), since torch's allocator would not
-    know that the stream uses it."""
+    of its own, from the graph's memory; for a raw stream handle none: the
+    library's own of that stream, which it refuses under capture."""
     if stream is not None:
         return None, None, 0
     if torch.cuda.is_current_stream_capturing():

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._tensors import Workspaces
+from ._tensors import Workspaces, run_on, stream_argument
 from .qformats import BLOCK_BYTES, QK
 
 _SOA_FN = {"q8_0": "qgemv_q8_0_soa", "q4_0": "qgemv_q4_0_soa"}
@@ -26,11 +26,17 @@ _AOS_FN = {"q8_0": "qgemv_q8_0_aos", "q4_0": "qgemv_q4_0_aos"}
 def _on_tensor_device(fn):
     """Runs ``fn`` with the device of its first CUDA tensor argument current:
     the C ABI launches on the current device, and the per-device state it
-    keeps (workspaces, tile counters) belongs to that device too."""
+    keeps (workspaces, tile counters) belongs to that device too.  With a raw
+    ``stream`` that stream is current as well."""
+    stream_of_call = stream_argument(fn)
+
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
         for a in (*args, *kwargs.values()):
             if isinstance(a, torch.Tensor) and a.is_cuda:
+                stream = stream_of_call(args, kwargs)
+                if stream is not None:
+                    return run_on(stream, a.device.index, fn, args, kwargs)
                 with torch.cuda.device(a.device):
                     return fn(*args, **kwargs)
         return fn(*args, **kwargs)
@@ -75,8 +81,8 @@ _WS = Workspaces()
 def _workspace(device, nbytes: int, stream) -> torch.Tensor:
     """A device buffer of at least ``nbytes`` for a call on the current torch
     stream (``stream`` None).  Under stream capture, or for a raw stream
-    handle, a fresh buffer from torch's caching allocator (stream-ordered; a
-    captured graph keeps its own)."""
+    handle (which is current here), a fresh buffer from torch's caching allocator
+    (stream-ordered; a captured graph keeps its own)."""
     nbytes = max(int(nbytes), 16)
     cur = torch.cuda.current_stream(device)
     if stream is not None or torch.cuda.is_current_stream_capturing():
