@@ -65,6 +65,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
   return true;
 }
+// The same by a whole warp, which goes on or gives up as one: a lane may see
+// the barrier, another the abort flag, and what follows (elections, TMEM loads,
+// shuffles, barriers of the CTA) wants every lane.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
 // Wait for copies and MMAs in flight before the CTA exits (they complete on
 // their own): ignores the abort flag, bounded by at least the default limit.
 __device__ __forceinline__ void mbar_wait_drain(uint32_t bar, uint32_t parity) {
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
       for (int i = 0; i < pre; ++i) load_x(i);
       int issued = pre;
       for (int i = pre; i < steps; ++i) {
-        if (!__all_sync(0xffffffffu, mbar_wait(saddr(&empty[i % S]), (uint32_t)((i / S - 1) & 1), &abort_flag))) break;
+        if (!warp_wait(saddr(&empty[i % S]), (uint32_t)((i / S - 1) & 1), &abort_flag)) break;
         load_w(i);
         load_x(i);
         issued = i + 1;
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
     bool ok = true;
     for (int i = 0; i < steps && ok; ++i) {
       const int s = i % S;
-      ok = __all_sync(0xffffffffu, mbar_wait(saddr(&full[s]), (uint32_t)((i / S) & 1), &abort_flag));
+      ok = warp_wait(saddr(&full[s]), (uint32_t)((i / S) & 1), &abort_flag);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -393,8 +399,7 @@ __global__ void __launch_bounds__(I8_THREADS) k_int8_mm(const __grid_constant__ 
     for (int c = threadIdx.x - 64; c < nn; c += 128) xs_s[c] = p.xs[n0 + c];
     const float ws = m < p.M ? p.ws[m] : 0.0f, b = m < p.M && p.bias ? p.bias[m] : 0.0f;
     asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
-    mbar_wait(saddr(&done), 0u, &abort_flag);
-    __syncwarp();
+    warp_wait(saddr(&done), 0u, &abort_flag);  // given up or not: the rest is in bounds
     tc_fence_after();
     const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16);
     if (cs > 1) {
@@ -551,7 +556,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       uint32_t phase = 0u;
       int m0 = m_of(at.t), n0 = n_of(at.t);
       while (issued < total) {
-        if (!__all_sync(0xffffffffu, mbar_wait(saddr(&empty[at.s]), phase, &abort_flag))) break;
+        if (!warp_wait(saddr(&empty[at.s]), phase, &abort_flag)) break;
         if (at.k == 0) {
           m0 = m_of(at.t);
           n0 = n_of(at.t);
@@ -583,12 +588,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       uint32_t phase = 0u;
       for (; t < mine && ok; ++t) {
         const int b = t & 1;
-        if (t >= 2) ok = mbar_wait(saddr(&tempty[b]), (uint32_t)((t / 2 - 1) & 1), &abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        if (t >= 2) ok = warp_wait(saddr(&tempty[b]), (uint32_t)((t / 2 - 1) & 1), &abort_flag);
         tc_fence_after();
         for (int k = 0; k < p.nk && ok; ++k) {
-          ok = mbar_wait(saddr(&full[s]), phase, &abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = warp_wait(saddr(&full[s]), phase, &abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -632,8 +635,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PR_THREADS, 1)
       for (int c = lane; c < nn; c += 32) xs[c] = p.xs[n0 + c];
       const float ws = m < p.M ? p.ws[m] : 0.0f, bv = m < p.M && p.bias ? p.bias[m] : 0.0f;
       __syncwarp();
-      if (!mbar_wait(saddr(&tfull[b]), (uint32_t)((t / 2) & 1), &abort_flag)) break;
-      __syncwarp();
+      if (!warp_wait(saddr(&tfull[b]), (uint32_t)((t / 2) & 1), &abort_flag)) break;
       tc_fence_after();
       store_cols<Y, PR_N / 2>(tmem + ((uint32_t)(quarter * 32) << 16) + b * PR_N + half * hw, nn, xs, ws, bv,
                               static_cast<Y*>(p.y) + (int64_t)n0 * p.ldy + m - lane, p.ldy, p.M - m + lane, lane);

@@ -797,6 +797,12 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile i
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_try(bar, parity) || wait_slow(bar, parity, abort_flag);
 }
+// The same by a whole warp, which goes on or gives up as one: a lane may see
+// the barrier, another the abort flag, and what follows (warp-wide reductions,
+// shuffles and MMAs, the cluster's barrier) wants every lane.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
 // Wait for a copy in flight before the CTA ends: ignores the abort flag,
 // bounded by at least the default limit.
 __device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
@@ -1179,7 +1185,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       while (l < ns) {
         al += MOE_KS;
         const auto next = peek();
-        if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
+        if (!warp_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
         w.slab(saddr(up_smem) + turn.s * slab_bytes<FMT>(), rt, now, next, lane);
         __syncwarp();  // every lane has read the stage
         if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
@@ -1198,7 +1204,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       pos = ran;
       l0 = first_slab(l0);
       l = l0;
-      if (j >= 2 && !mbar_wait(saddr(&pipe.pempty[b]), (uint32_t)(j / 2 - 1) & 1u, &pipe.abort_flag)) break;
+      if (j >= 2 && !warp_wait(saddr(&pipe.pempty[b]), (uint32_t)(j / 2 - 1) & 1u, &pipe.abort_flag)) break;
       w.each((en >> 22) & 15, lane, [&](int i, float gate, float up) {
         float* p = part.v[b][kq][i] + rt * 8 + (lane >> 2);
         p[0] = gate;
@@ -1215,7 +1221,7 @@ __global__ void __launch_bounds__(UP_THREADS, 1) k_moe_up(MoeArgs a) {
       int hb;  // the unit's block of h
       const uint32_t en = unit(hb);
       const int at = (en >> 10) & 0xFFF, cnt = (en >> 22) & 15, b = j & 1;
-      if (!mbar_wait(saddr(&pipe.pfull[b]), (uint32_t)(j / 2) & 1u, &pipe.abort_flag)) break;
+      if (!warp_wait(saddr(&pipe.pfull[b]), (uint32_t)(j / 2) & 1u, &pipe.abort_flag)) break;
       for (int i = warp - MOE_CW - 1; i < cnt; i += MOE_EW) {
         float gate = 0.0f, up = 0.0f;
 #pragma unroll
@@ -1319,7 +1325,7 @@ __global__ void __launch_bounds__(DN_THREADS, 1) k_moe_down(MoeArgs a, int ydt) 
         }
         next = w.ahead(al * SG, min(SG, fg - al * SG));
       }
-      if (!mbar_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
+      if (!warp_wait(saddr(&pipe.full[turn.s]), turn.phase, &pipe.abort_flag)) break;
       w.slab(saddr(dn_smem) + turn.s * slab_bytes<FMT>(), rt, now, next, lane);
       __syncwarp();  // every lane has read the stage
       if (lane == 0) mbar_arrive(saddr(&pipe.empty[turn.s]));
