@@ -450,6 +450,8 @@ __global__ void __launch_bounds__(TcFmt<FMT, NC>::THREADS, 1)
       ok = mbar_wait(saddr(&full[s]), (uint32_t)((i / SW) & 1), &abort_flag);
       if (ok && i >= C::SA)
         ok = mbar_wait(saddr(&aempty[i % C::SAD]), (uint32_t)(((i / C::SAD) - 1) & 1), &abort_flag);
+      // the warp goes on or gives up as one: its lanes meet below
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();  // the A slot was last read by MMAs (async proxy)
       const uint8_t* pk = ring + (size_t)s * C::WSTAGE;

@@ -30,3 +30,10 @@ def test_a_warp_gives_up_as_one(name):
             assert rest[:m.start()].rstrip().endswith("if (lane == 0) {")
     assert not single, [rest[i:i + 60] for i in single]
     assert len(re.findall(r"(?<!bool )\bwarp_wait\(", rest)) >= 4
+
+
+def test_the_q4_converters_give_up_as_one():
+    """gemv_tc.cu: the converter warps' waits, whose loop holds a __syncwarp."""
+    text = code("gemv_tc.cu")
+    part = text[text.index("(i / C::SAD) - 1) & 1)"):]
+    assert re.match(r"[^;]*;\s*ok = __all_sync\(0xffffffffu, ok\);\s*if \(!ok\) break;", part)
