@@ -613,7 +613,7 @@ QGEMV_API int qgemv_moe_layer(const qgemv_expert_set* experts, const qgemv_moe_r
 /* One scale per row: scales = max |x| / 127, q = rint(x / scales) (fp32
  * division and rounding), for activations and weights alike.  An all-zero row
  * gets scale 0 and zeros, a row with a NaN or an infinity scale NaN and zeros
- * (its products are NaN).  Any K; row n of x at x + n * ldx elements, of q at
+ * (its products are NaN).  K below 2^31 - 512; row n of x at x + n * ldx elements, of q at
  * q + n * ldq bytes. */
 QGEMV_API int qgemv_int8_quantize(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t K,
                                   void* q, int64_t ldq, float* scales, void* stream);

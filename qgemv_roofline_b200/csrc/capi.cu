@@ -1134,7 +1134,9 @@ QGEMV_API int qgemv_int8_quantize(const void* x, int dtype, int64_t ldx, int64_t
                                   void* q, int64_t ldq, float* scales, void* stream) {
   if (dtype < 0 || dtype > 2) return set_error(ERR_ARG, "dtype must be 0, 1 or 2, got %d", dtype);
   if (rows < 0 || K < 1) return set_error(ERR_SHAPE, "rows=%lld K=%lld", (long long)rows, (long long)K);
-  if (rows >= kMaxDim || K >= kMaxDim - 16) return set_error(ERR_UNSUPPORTED, "rows and K must be below 2^31");
+  if (rows >= kMaxDim || K >= kMaxDim - 512)  // a row's columns are counted in 32 bits, 256 at a time
+    return set_error(ERR_UNSUPPORTED, "rows must be below 2^31 and K below 2^31 - 512 (rows=%lld K=%lld)",
+                     (long long)rows, (long long)K);
   if (rows == 0) return OK;
   if (!x || !q || !scales) return set_error(ERR_NULL, "x, q and scales must not be NULL");
   if (misaligned(x, dtype == 0 ? 4 : 2) || misaligned(scales, 4))
