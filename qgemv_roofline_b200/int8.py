@@ -38,8 +38,8 @@ def quantize_int8(x: torch.Tensor, q: torch.Tensor | None = None, scales: torch.
     vec = x.dim() == 1
     if q is None:
         q = new(x.shape, torch.int8, x.device)
-    elif q.dtype != torch.int8 or q.shape != x.shape or q.device != x.device or q.stride(-1) != 1 or \
-            (not vec and N > 1 and q.stride(0) < K):
+    elif q.dtype != torch.int8 or q.shape != x.shape or q.device != x.device or \
+            (q.stride(-1) != 1 and K > 1) or (not vec and N > 1 and q.stride(0) < K):
         raise ValueError("q must be an int8 tensor like x with unit last stride")
     want = x.shape[:-1]
     if scales is None:

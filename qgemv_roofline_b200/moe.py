@@ -34,7 +34,7 @@ def _router(router, top_k, scoring, bias, scale, normalize, device) -> _lib.MoeR
         raise ValueError(f"router must be a float32, bfloat16 or float16 tensor [E, K] on {device}")
     ldw, last = router.stride()
     E = shape[0]
-    if last != 1 or (E > 1 and ldw < shape[1]):
+    if (last != 1 and shape[1] > 1) or (E > 1 and ldw < shape[1]):
         raise ValueError("router must have unit last stride and rows that do not overlap")
     if scoring not in SCORING:
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
