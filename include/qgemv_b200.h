@@ -575,7 +575,9 @@ typedef struct qgemv_moe_router {
 
 /* Routing alone: ids int32 [N][top_k] in descending order of score, weights
  * fp32 [N][top_k].  Equal scores go to the lower index; a NaN score ranks
- * below every number, and a token with a NaN logit gets NaN weights. */
+ * below every number, and a token with a NaN logit gets NaN weights.  Scores
+ * are fp32 numbers: a sigmoid of a logit below about -88.7 is 0, and where all
+ * chosen scores are 0 so are the weights, normalised or not. */
 QGEMV_API int qgemv_moe_route(const qgemv_moe_router* router, const void* x, int dtype,
                               int64_t ldx, int64_t n_tokens, int64_t hidden, int32_t* ids,
                               float* weights, void* stream);

@@ -350,15 +350,21 @@ __device__ void route_token(const RouteArgs& r, const float* logit, unsigned lon
     __syncwarp();
     mine = pick(key, E, r.k, lane);
   }
-  float s = 0.0f;
+  float s = 0.0f, top = mx;
+  if (r.bias && r.normalize && r.scoring == 0) {
+    // the bias may have chosen experts far below the best one: their weights
+    // are relative to each other, so to the largest of them
+    float c = lane < r.k ? logit[mine] : -INFINITY;
+    for (int o = 16; o; o >>= 1) c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, o));
+    if (c != -INFINITY) top = c;
+  }
   if (lane < r.k) {
     const float l = logit[mine];
-    s = r.scoring == 0 ? expf(l - mx) : 1.0f / (1.0f + expf(-l));
+    s = r.scoring == 0 ? expf(l - top) : 1.0f / (1.0f + expf(-l));
   }
   const float sum = warp_sum(s);
-  // a sum below the smallest normal number (every chosen score underflowed)
-  // divides as that number: weights of zero, not NaN
-  float den = r.normalize ? fmaxf(sum, 1.17549435e-38f) : 1.0f;
+  // scores are fp32 numbers: where every chosen one is 0 the weights are, not NaN
+  float den = r.normalize && sum > 0.0f ? sum : 1.0f;
   if (!r.normalize && r.scoring == 0) {
     float all = 0.0f;
     for (int e = lane; e < E; e += 32) all += expf(logit[e] - mx);
