@@ -56,3 +56,31 @@ def test_chosen_experts_of_no_score():
     r = torch.tensor([[0.0, 1.0], [-1e30, 0.0], [-1e30, 0.0]], device=DEV)
     ids, w = qg.moe_route(x, r, 2, bias=torch.tensor([0.0, 2.0, 2.0], device=DEV))
     assert ids.tolist() == [[1, 2]] * 2 and (w == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TORCH))
+@pytest.mark.parametrize("rdtype", list(TORCH))
+@pytest.mark.parametrize("N,E,K", [(33, 20, 90), (50, 37, 256), (129, 300, 131), (40, 9, 7)])
+def test_many_tokens_by_type_and_stride(dtype, rdtype, N, E, K):
+    """Both matrices in vectors (rows of 16-byte multiples) and by element."""
+    rng = np.random.default_rng(N + E)
+    x = torch.from_numpy(rng.standard_normal((N, K)).astype(np.float32)).to(TORCH[dtype])
+    r = torch.from_numpy((2 * K ** -0.5 * rng.standard_normal((E, K))).astype(np.float32)).to(TORCH[rdtype])
+    for xo, ro, pad in ((0, 0, 0), (3, 0, 8), (0, 5, 9), (8, 8, 24)):
+        xt, rt = (torch.full((t.shape[0], K + pad + o), float("nan"), dtype=t.dtype, device=DEV)
+                  for t, o in ((x, xo), (r, ro)))
+        xt[:, xo:xo + K], rt[:, ro:ro + K] = x.to(DEV), r.to(DEV)
+        check(x.float().numpy(), r.float().numpy(), min(5, E), xt=xt[:, xo:xo + K], rt=rt[:, ro:ro + K])
+
+
+@pytest.mark.parametrize("N", [1, 2, 7, 35])
+@pytest.mark.parametrize("E,K", [(8, 5120), (160, 4100), (1024, 96), (700, 2052), (300, 7168), (1, 9000), (5, 4097)])
+@pytest.mark.parametrize("dtype,rdtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "bfloat16")])
+def test_long_rows_and_many_experts(N, E, K, dtype, rdtype):
+    """Rows longer than a staged chunk of x (4096 or 2048 columns), more tiles of experts than warps."""
+    rng = np.random.default_rng(N + E + K)
+    x = torch.from_numpy(rng.standard_normal((N, K)).astype(np.float32)).to(TORCH[dtype])
+    r = torch.from_numpy((2 * K ** -0.5 * rng.standard_normal((E, K))).astype(np.float32)).to(TORCH[rdtype])
+    bias = (rng.random(E) * 0.2).astype(np.float32)
+    for scoring, b in (("softmax", None), ("sigmoid", bias)):
+        check(x.float().numpy(), r.float().numpy(), min(E, 8), scoring, b, 2.5, xt=x.to(DEV), rt=r.to(DEV))
