@@ -101,7 +101,10 @@ __device__ __noinline__ uint32_t quant_exact(float v, float s) {
 constexpr int RQ_THREADS = 256;
 constexpr int RQ_HELD = 2;  // vectors of 8 values that a thread keeps
 
-// One CTA per row.  A row with a NaN or an infinity gets the scale NaN and
+// One CTA per row.  4096 rows of 4096 in bf16: 16.4 us (50 MB, 7.7 at the copy
+// rate), 2.8 of 4 instructions per cycle with half the warps: issue and, at the
+// barrier between reading and writing, the loads' latency.  A single row is a
+// launch and two round trips (4.8 us alone).  A row with a NaN or an infinity gets the scale NaN and
 // zeros; an all-zero row (or one whose scale underflows to 0) the scale 0 and
 // zeros.  VEC: rows start on 16-byte boundaries, q's on 8-byte ones, and K is a
 // multiple of 8: a row of up to 4096 values is read once and kept.
@@ -200,7 +203,11 @@ struct I8Args {
   void* y;
   int64_t ldy;
   int M, N, nk;    // nk: K steps
-  int early_w;     // the weights may be read before the dependency wait
+  // The weights may be read before the dependency wait: the launch before this
+  // one is the row kernel of the same call, every CTA of which had waited for
+  // what came before it when this launch was allowed; the copies read L2, where
+  // those writes are by then.
+  int early_w;
 };
 
 constexpr int I8_CL = 8;  // CTAs of a cluster at most

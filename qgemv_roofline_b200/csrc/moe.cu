@@ -29,15 +29,16 @@
 // compute warps, one per row tile and one of three splits: split s takes every
 // third slab.  Every wait is bounded.  What bounds them (one B200; the copy rate
 // is 6.54 TB/s): with few tokens per expert q8_0 the weights' stream (16 tokens,
-// 64 + 2 experts of 4096x1408: 971 MB in 178 us, 0.83 of the copy rate); q4_0 with
-// several tokens the instructions per 16 x 32 weights (42 against the 50 that the
-// stream leaves room for, at 0.6 to 0.8 issued per cycle: 64 tokens, 128 experts of
-// 2048x768, 335 MB in 105 us, 0.49); a single token the launches' latencies (128
-// experts of 2048x768 in q4_0, 8 chosen, 22 MB: 20 us, of which routing 8, entries
-// and first copies 2 x 2, the two products' slabs 5).  Tried and slower: 16 compute
-// warps of 96 registers (64 tokens 105 -> 156 us, spills), four MMAs of tokens per
-// entry (spills), units of their own for the splits (64 tokens 105 -> 103 us, one
-// token 20 -> 22), private rings of 16 warps without a producer (149 us).
+// 64 + 2 experts of 4096x1408: 971 MB in 192 us, 0.77 of the copy rate); q4_0 with
+// several tokens the latency of a slab's digits and shared-memory loads, with four
+// warps a scheduler (64 tokens, 128 experts of 2048x768, 335 MB in 159 us, 0.32:
+// gate / up at 2.3 of 4 instructions per cycle, stalled on loads for 2.1 cycles per
+// instruction and on fixed latencies for 1.5, down at 1.8); a single token the
+// launches' latencies (128 experts of 2048x768 in q4_0, 8 chosen, 22 MB: 21.7 us).
+// Tried and slower, when 16-bit types had two digits: 16 compute warps of 96
+// registers (64 tokens 105 -> 156 us, spills), four MMAs of tokens per entry
+// (spills), units of their own for the splits (64 tokens 105 -> 103 us, one token
+// 20 -> 22), private rings of 16 warps without a producer (149 us).
 //
 // The arithmetic is the library's exact-integer scheme.  A block of 32
 // activations is rounded to integers X = rint(x FX / max |x|) and split into
