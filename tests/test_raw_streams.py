@@ -16,16 +16,9 @@ DEV = "cuda"
 @pytest.mark.parametrize("wrap", [_tensors.on_device_of_x, gemv._on_tensor_device])
 @pytest.mark.parametrize("handle,positional", [(9, False), (9, True), (0, False), (5, False), (None, False)])
 def test_the_raw_stream_is_current_inside_the_call(wrap, handle, positional, monkeypatch):
-    """Stand-ins for torch's streams: no GPU."""
+    """Stand-ins for torch's streams (a stream's id is its handle): no GPU."""
     current, used = [5], []
-    stream = lambda h, device=None: types.SimpleNamespace(cuda_stream=h)
-
-    @contextlib.contextmanager
-    def enter(s):
-        current.append(s.cuda_stream)
-        yield
-        current.pop()
-
+    stream = lambda h, device=None: types.SimpleNamespace(stream_id=h, device_index=0, device_type=1)
     class Tensor(torch.Tensor):
         is_cuda, device = True, types.SimpleNamespace(index=0)
 
@@ -33,25 +26,37 @@ def test_the_raw_stream_is_current_inside_the_call(wrap, handle, positional, mon
             return 0
 
         def record_stream(self, s):
-            used.append(s.cuda_stream)
+            used.append(s)
 
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: stream(current[-1]))
     monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: stream(0))
     monkeypatch.setattr(torch.cuda, "ExternalStream", stream)
-    monkeypatch.setattr(torch.cuda, "stream", enter)
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     monkeypatch.setattr(_tensors, "_current_device", lambda: 0)
+    monkeypatch.setattr(_tensors, "_raw_stream", lambda index: current[-1])
+    monkeypatch.setattr(_tensors, "_get_stream", lambda index: (current[-1], index, 1))
+    monkeypatch.setattr(_tensors, "_set_stream", lambda s: current.append(s[0]))
+    monkeypatch.setattr(_tensors, "_stream_object", lambda h, index, kind: h)
+    _tensors._stream_of_handle.cache_clear()
     x = torch.zeros(2).as_subclass(Tensor)
     seen = []
 
     @wrap
     def call(x, y=None, stream=None):
-        seen.append(torch.cuda.current_stream().cuda_stream)
-        return x
+        seen.append(current[-1])
+        if y is not None and (y == 7).all():
+            raise ValueError
+        return torch.zeros(2).as_subclass(Tensor) if y is None else y
 
     call(x, None, handle) if positional else call(x, stream=handle)
-    assert seen == [5 if handle is None else handle] and current == [5]
-    assert used == ([5] if handle in (0, 9) else [])  # the result waits for the caller's stream, too
+    here = 5 if handle is None else handle
+    assert seen == [here] and current[-1] == 5
+    assert used == ([5] if handle in (0, 9) else [])  # a new result waits for the caller's stream, too
+    y = torch.zeros(2).as_subclass(Tensor)
+    assert call(x, y, stream=handle) is y and used == ([5] if handle in (0, 9) else [])
+    with pytest.raises(ValueError):
+        call(x, y + 7, stream=handle)
+    assert seen == [here] * 3 and current[-1] == 5  # whatever the call does
+    _tensors._stream_of_handle.cache_clear()
 
 
 def calls():
